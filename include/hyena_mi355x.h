@@ -11,7 +11,7 @@
  *   - return 0 on success, a negative HYENA_E* for a rejected argument,
  *     a positive hipError_t if the launch failed; hyena_last_error_string()
  *     describes the last failure on the calling thread.
- * All activation tensors are bfloat16.  Filters, biases, poles are float32.
+ * All activation tensors are bfloat16 unless an entry point takes a dtype.  Filters, biases, poles are float32.
  */
 #ifndef HYENA_MI355X_H
 #define HYENA_MI355X_H
@@ -385,7 +385,8 @@ int hyena_fir_cl_fwd(const hyena_cl* x1, const hyena_cl* x2, const hyena_cl* v,
 enum hyena_dtype {
     HYENA_DTYPE_BF16 = 0,
     HYENA_DTYPE_F16 = 1,
-    HYENA_DTYPE_F32 = 2
+    HYENA_DTYPE_F32 = 2,
+    HYENA_DTYPE_F8E4M3 = 3      /* OCP e4m3 (finite, +-448): key / value pages only */
 };
 
 /* hyena_fir_cl_fwd for the element types the reference's own parity grid of this operator runs in
@@ -444,6 +445,81 @@ int hyena_fir_layer_fwd(const hyena_proj_fwd* proj,
                         const float* h, int taps_reversed, const float* bias, int bias_mode,
                         void* out, void* bx_out, int64_t bx_from,
                         int64_t B, int64_t L, int64_t D, int64_t G, int K, void* stream);
+
+/* ---- Paged key / value cache of the attention blocks -------------------------------------------------------------
+ *
+ * The reference's attention blocks keep one [B, max_seqlen, 2, H, head_dim] tensor per layer (vortex/model/cache.py:8-28)
+ * or a paged cache addressed through a block table (vortex/ops/attn_interface.py, flash_attn_with_kvcache).  Here a
+ * layer's cache is pages of `page_size` positions: element (page, head, slot, d) of a side sits at
+ *   ptr + page*page_stride + head*head_stride + slot*slot_stride + d         (strides in elements, d contiguous),
+ * and position j of sequence s lives in page table[s*table_stride + j / page_size], slot j % page_size.
+ * `scale` [kv_heads] float32 (or NULL for 1): what a stored value is multiplied by; e4m3 pages use it.
+ * A page id outside 0..num_pages-1 names no page: nothing is read from or written to it (attention leaves its positions
+ * out, an append drops them), and so do positions beyond table_width*page_size.
+ * Rules (others: HYENA_ENOSUP / HYENA_EALIGN): head_dim a multiple of 8 up to 256; page_size a power of two from 16 to
+ * 65536; strides multiples of 8 elements, pointers 16-byte aligned. */
+typedef struct hyena_kv_side {
+    void* ptr;
+    int64_t page_stride, head_stride, slot_stride;
+    const float* scale;
+} hyena_kv_side;
+
+typedef struct hyena_kv_pages {
+    hyena_kv_side k, v;
+    int64_t num_pages, page_size, kv_heads, head_dim;
+    const int32_t* table;
+    int64_t table_stride, table_width, sequences;
+    int dtype;                  /* of the pages: BF16 / F16 (the activations' type) or F8E4M3 */
+    int reserved;               /* 0 */
+} hyena_kv_pages;
+
+/* Token rows [tokens][heads][head_dim]; a NULL ptr means "absent" where that is allowed. */
+typedef struct hyena_heads {
+    void* ptr;
+    int64_t token_stride, head_stride;
+} hyena_heads;
+
+/* Attention of ONE new token per sequence over its cached positions 0..lens[s]-1 (the token's own key among them: append
+ * first).  Replaces the cached single-token branch of vortex/model/attention.py (flash_attn_with_kvcache / the
+ * non-flash products :247-283).  For head h of sequence s, with g = heads / kv_heads:
+ *   w_j = exp(scale * k.scale[h/g] * <q, K_j> - max),  out = v.scale[h/g] * sum_j w_j V_j / sum_j w_j
+ * q [sequences][heads][head_dim] (token_stride = sequence stride), out the same, contiguous, of the type of q (`dtype`:
+ * BF16 or F16).  lens[s] <= 0 gives zeros; lens[s] beyond the table's reach counts as its reach.  Values behind
+ * lens[s] in a page may be anything, NaN included.  Sums and softmax statistics are float32.
+ * ws: hyena_attn_step_ws_bytes(sequences, heads, kv_heads, head_dim) bytes of device memory for the parts of long
+ * sequences, contents of no interest before and after; calls that overlap in time need one each. */
+int64_t hyena_attn_step_ws_bytes(int64_t sequences, int64_t heads, int64_t kv_heads, int64_t head_dim);
+int hyena_attn_step(const hyena_kv_pages* kv, const hyena_heads* q, const int32_t* lens, float scale, void* out,
+                    void* ws, int64_t ws_bytes, int64_t heads, int dtype, void* stream);
+
+/* Rotary positions of q and k (vortex/ops/embedding/rotary.py:12-221, vortex/model/rotary.py) and the append of k and v
+ * to the pages, in one pass.  Row t of q [tokens][heads][head_dim], k, v [tokens][kv_heads][head_dim] belongs to sequence
+ * seq[t], or t / (tokens / sequences) when seq == NULL, at position pos[t]; pair i of a head, (x[i], x[i + rotary_dim/2])
+ * or with interleaved (x[2i], x[2i+1]), turns by pos[t]*turns[i] revolutions:
+ *   y1 = x1 cos - x2 sin,  y2 = x1 sin + x2 cos
+ * in float32, the angle in float64 (reduced before the cosine); dimensions from rotary_dim on pass unchanged.
+ * turns [rotary_dim/2] float64: 1 / (2 pi base^(2i/rotary_dim)) for plain rotary embedding, divided by the factor for
+ * interpolated positions, or any other table.  q_out and k_out (optional) get the rotated rows in the activations'
+ * type; q_out may be q, k_out may be k.  Pages of the activations' type get the same values as k_out; e4m3 pages get
+ * k / scale, v / scale, clamped to +-448, in one rounding from float32.
+ * pos[t] < 0 marks a padding row: nothing of it is written (with zero_skipped != 0 its row of q_out becomes
+ * zeros).  A sequence or position outside the table writes no page.  Two rows with the same sequence and position are the
+ * caller's mistake: one of them stays. */
+int hyena_rotary_append(const hyena_kv_pages* kv, const hyena_heads* q, const hyena_heads* k, const hyena_heads* v,
+                        const hyena_heads* q_out, const hyena_heads* k_out, const int32_t* pos, const int32_t* seq,
+                        const double* turns, int64_t rotary_dim, int interleaved, int zero_skipped,
+                        int64_t tokens, int64_t heads, int dtype, void* stream);
+
+/* Copies pages: for every pool n < pools and pair i < copies, page_bytes bytes from page src[i] of src_pools to page
+ * dst[i] of dst_pools.  Page p of pool n starts at base + n*pool_stride + p*page_stride (bytes).  src_pools and dst_pools
+ * may be the same memory (fork, compaction): then no page may be both a source and a destination, and either way no
+ * destination may come twice.  A pair with a page outside 0..src_pages-1 / 0..dst_pages-1 is left out. */
+typedef struct hyena_kv_pools {
+    void* base;
+    int64_t pool_stride, page_stride, pages;
+} hyena_kv_pools;
+int hyena_kv_copy_pages(const hyena_kv_pools* src_pools, const hyena_kv_pools* dst_pools, int64_t pools,
+                        int64_t page_bytes, const int32_t* src, const int32_t* dst, int64_t copies, void* stream);
 
 #ifdef __cplusplus
 }

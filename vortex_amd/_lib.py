@@ -4,13 +4,13 @@ There is no fallback: if the library is missing, every operator raises.
 """
 import ctypes
 import os
-from ctypes import POINTER, Structure, c_char_p, c_int, c_int64, c_void_p
+from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int64, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libhyena_mi355x.so")
 
 HYENA_BIAS_NONE, HYENA_BIAS_ADD, HYENA_BIAS_GATED_FP32, HYENA_BIAS_ADD_FP32, HYENA_BIAS_GATED_BF16 = 0, 1, 2, 3, 4
-HYENA_DTYPE_BF16, HYENA_DTYPE_F16, HYENA_DTYPE_F32 = 0, 1, 2
+HYENA_DTYPE_BF16, HYENA_DTYPE_F16, HYENA_DTYPE_F32, HYENA_DTYPE_F8E4M3 = 0, 1, 2, 3
 
 EXPORTS = [
     "hyena_version", "hyena_last_error_string", "hyena_se_fwd", "hyena_mr_fwd",
@@ -21,6 +21,7 @@ EXPORTS = [
     "hyena_fir_far_period", "hyena_fir_far_bytes", "hyena_fir_step_far", "hyena_fir_layer_step_far",
     "hyena_iir_window_tokens", "hyena_iir_window_supported", "hyena_iir_step_win", "hyena_iir_layer_step_win",
     "hyena_iir_window_flush",
+    "hyena_attn_step_ws_bytes", "hyena_attn_step", "hyena_rotary_append", "hyena_kv_copy_pages",
 ]
 
 
@@ -52,6 +53,29 @@ class ProjFwd(Structure):
     _fields_ = [("u", c_void_p), ("u_batch_stride", c_int64), ("u_time_stride", c_int64), ("w", c_void_p),
                 ("bias", c_void_p), ("Ks", c_int), ("flip_x1x2", c_int), ("ch_inner", c_int64), ("ch_outer", c_int64),
                 ("gate_stride", c_int64), ("ch_stride", c_int64)]
+
+
+class KvSide(Structure):
+    """hyena_kv_side: the pages of the keys or of the values."""
+    _fields_ = [("ptr", c_void_p), ("page_stride", c_int64), ("head_stride", c_int64), ("slot_stride", c_int64),
+                ("scale", c_void_p)]
+
+
+class KvPages(Structure):
+    """hyena_kv_pages: one layer's paged key / value cache and the page table of the sequences."""
+    _fields_ = [("k", KvSide), ("v", KvSide), ("num_pages", c_int64), ("page_size", c_int64), ("kv_heads", c_int64),
+                ("head_dim", c_int64), ("table", c_void_p), ("table_stride", c_int64), ("table_width", c_int64),
+                ("sequences", c_int64), ("dtype", c_int), ("reserved", c_int)]
+
+
+class HeadRows(Structure):
+    """hyena_heads: token rows [tokens][heads][head_dim]."""
+    _fields_ = [("ptr", c_void_p), ("token_stride", c_int64), ("head_stride", c_int64)]
+
+
+class KvPools(Structure):
+    """hyena_kv_pools: pools of pages of one size."""
+    _fields_ = [("base", c_void_p), ("pool_stride", c_int64), ("page_stride", c_int64), ("pages", c_int64)]
 
 
 _lib = None
@@ -126,10 +150,17 @@ def lib():
     L.hyena_featurizer_gates_fwd.argtypes = [POINTER(ProjFwd), c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p]
     L.hyena_fir_layer_fwd.argtypes = [POINTER(ProjFwd), c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int64,
                                       c_int64, c_int64, c_int64, c_int64, c_int, c_void_p]
+    KV, HR, KP = POINTER(KvPages), POINTER(HeadRows), POINTER(KvPools)
+    L.hyena_attn_step_ws_bytes.argtypes = [c_int64, c_int64, c_int64, c_int64]
+    L.hyena_attn_step.argtypes = [KV, HR, c_void_p, c_float, c_void_p, c_void_p, c_int64, c_int64, c_int, c_void_p]
+    L.hyena_rotary_append.argtypes = [KV, HR, HR, HR, HR, HR, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int64,
+                                      c_int64, c_int, c_void_p]
+    L.hyena_kv_copy_pages.argtypes = [KP, KP, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_void_p]
     for name in EXPORTS:
         fn = getattr(L, name)
         if name not in ("hyena_version", "hyena_last_error_string"):
-            fn.restype = c_int64 if name in ("hyena_li_plan_bytes", "hyena_fir_far_period", "hyena_fir_far_bytes", "hyena_iir_window_tokens") else c_int
+            fn.restype = c_int64 if name in ("hyena_li_plan_bytes", "hyena_fir_far_period", "hyena_fir_far_bytes", "hyena_iir_window_tokens",
+                                             "hyena_attn_step_ws_bytes") else c_int
     _lib = L
     return L
 
