@@ -1,7 +1,25 @@
 // Attention of one new token per sequence over a paged key / value cache.
+//
+//   s_j = scale * <q, K_j>,  o = sum_j 2^(s_j - m) V_j / sum_j 2^(s_j - m)     (scale includes log2 e)
+//
+// Bound by the bytes of K and V: one multiply-add per stored element and query head.  Everything is laid out so that
+// each wavefront streams pages through registers with no LDS and no barrier:
+//   * S^T = K Q^T on v_mfma_f32_16x16x32: a lane holds 8 consecutive elements of ONE key (16 bytes as they lie in the
+//     page), the columns are up to 16 query heads that share the key head;
+//   * the result leaves key 4*(lane/16) + i of a 16-key piece in register i of lane `lane`, column lane % 16 -- which is
+//     where the A operand of the next product wants the weights if its 32 keys are numbered (lane/16, piece, i).
+//     So the weights never move between lanes;
+//   * O = P V: a lane loads 8 consecutive elements of a value row for each of its 8 keys (full rows per 16 lanes) and
+//     pairs the keys up with one v_perm per two elements.
+// The weights go in as two 16-bit terms (hi + lo, 16 bits of mantissa): the products are free beside the loads, and the
+// output then differs from the float32 formula by the last rounding only.
+#include "kv_addr.h"
 #include "kv_cache.h"
 
 namespace {
+
+constexpr int WAVES = 4;                    // wavefronts of a block (they share nothing)
+constexpr float LAZY = 8.f;                 // the maximum follows the scores when one exceeds it by more than 2^8
 
 struct AttnArgs {
     KvPages kv;
@@ -9,70 +27,507 @@ struct AttnArgs {
     int64_t q_seq_stride, q_head_stride;    // bytes
     const int32_t* lens;
     char* out;
+    float* part_o;                          // [2 * wavefronts][rows of a tile][HDP]
+    float* part_ml;                         // [2 * wavefronts][rows of a tile][2]
     float scale;                            // includes log2(e): the softmax works in powers of two
-    int32_t heads, group;
+    int32_t heads, group, qtiles;           // query heads per key head, in tiles of 16
+    int32_t waves;
 };
 
-// One block per (sequence, head): 256 positions at a time, one score per thread, running maximum and sum.
-template <int DT, int KVDT>
-__global__ void __launch_bounds__(256) attn_step_kernel(AttnArgs a) {
-    typedef KvElem<DT> E;
-    typedef KvElem<KVDT> P;
-    typedef typename E::raw raw;
-    typedef typename P::raw praw;
-    __shared__ float q[256], p[256], red[256];
-    __shared__ const praw* vrow[256];
-    const int h = blockIdx.x % a.heads, b = blockIdx.x / a.heads, kh = h / a.group, tid = threadIdx.x, hd = a.kv.head_dim;
-    const int64_t n = min((int64_t)a.lens[b], a.kv.reach);
-    const int32_t* table = a.kv.table + b * a.kv.table_stride;
-    const float ks = a.scale * (a.kv.k.scale ? a.kv.k.scale[kh] : 1.f);
-    if (tid < hd) q[tid] = E::get(((const raw*)(a.q + b * a.q_seq_stride + h * a.q_head_stride))[tid]);
-    float m = -INFINITY, l = 0.f, acc = 0.f;
-    for (int64_t j0 = 0; j0 < n; j0 += 256) {
-        __syncthreads();
-        const int64_t j = j0 + tid;
-        float s = -INFINITY;
-        vrow[tid] = nullptr;
-        if (j < n) {
-            const int64_t page = table[j >> a.kv.page_shift], slot = j & ((1LL << a.kv.page_shift) - 1);
-            if (page >= 0 && page < a.kv.num_pages) {
-                const praw* k = (const praw*)(a.kv.k.ptr + page * a.kv.k.page_stride + kh * a.kv.k.head_stride + slot * a.kv.k.slot_stride);
-                vrow[tid] = (const praw*)(a.kv.v.ptr + page * a.kv.v.page_stride + kh * a.kv.v.head_stride + slot * a.kv.v.slot_stride);
-                float dot = 0.f;
-                for (int d = 0; d < hd; ++d) dot = fmaf(q[d], P::get(k[d]), dot);
-                s = dot * ks;
-            }
+template <int DT> struct Mma;
+template <> struct Mma<HYENA_DTYPE_BF16> {
+    static __device__ __forceinline__ f32x4 dot(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf2(lo, hi); }
+    // weights x, y >= 0 as head (cut off, not rounded) + rest; the rest is never 0, so that a weight times an
+    // infinite value stays infinite instead of adding 0 * inf
+    static __device__ __forceinline__ void split(float x, float y, uint32_t& head, uint32_t& rest) {
+        head = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
+        rest = pack(fmaxf(x - bf_lo(head), 0x1p-100f), fmaxf(y - bf_hi(head), 0x1p-100f));
+    }
+    template <bool HI> static __device__ __forceinline__ uint32_t from_f8(uint32_t w) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, HI));
+    }
+};
+template <> struct Mma<HYENA_DTYPE_F16> {
+    typedef __attribute__((__vector_size__(2 * sizeof(_Float16)))) _Float16 h2;
+    static __device__ __forceinline__ f32x4 dot(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        const h2 h = {(_Float16)lo, (_Float16)hi};
+        return __builtin_bit_cast(uint32_t, h);
+    }
+    static __device__ __forceinline__ void split(float x, float y, uint32_t& head, uint32_t& rest) {
+        const auto h = __builtin_amdgcn_cvt_pkrtz(x, y);
+        head = __builtin_bit_cast(uint32_t, h);
+        rest = pack(fmaxf(x - (float)h[0], 0x1p-24f), fmaxf(y - (float)h[1], 0x1p-24f));
+    }
+    template <bool HI> static __device__ __forceinline__ uint32_t from_f8(uint32_t w) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, HI));
+    }
+};
+
+__device__ __forceinline__ int lane_id() { return __lane_id(); }
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x), hi = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32));
+    return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ float max_over_keys(float x) {       // over the four lanes lane, lane ^ 16, ^ 32, ^ 48
+    x = fmaxf(x, __shfl_xor(x, 16));
+    return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ __forceinline__ float sum_over_keys(float x) {
+    x += __shfl_xor(x, 16);
+    return x + __shfl_xor(x, 32);
+}
+
+// Tiles of TK positions, in the order (sequence, key head, query tile, position); where a tile index falls.
+struct Place {
+    int64_t total;          // tiles of all sequences
+    int64_t waves;          // wavefronts that get some of them, one tile at least
+    int64_t first;          // tiles ahead of sequence b
+    int32_t b, tiles;       // the sequence and its tiles per (key head, query tile)
+};
+
+__device__ __forceinline__ int32_t seq_len(const AttnArgs& a, int32_t b) {
+    return (int32_t)min((int64_t)max(a.lens[b], 0), a.kv.reach);
+}
+
+// Sums the tiles of all sequences, 64 lengths at a time, and finds the sequence that holds the first tile of wavefront w,
+// or the one named by `want` where that is not negative.
+__device__ __forceinline__ Place find_place(const AttnArgs& a, int tk_shift, int32_t rows, int64_t w, int32_t want) {
+    const int lane = lane_id();
+    Place p = {0, 0, 0, 0, 0};
+    const int32_t B = a.kv.sequences;
+    for (int32_t b0 = 0; b0 < B; b0 += 64) {
+        int64_t t = 0;
+        if (b0 + lane < B) t = ((int64_t)seq_len(a, b0 + lane) + (1 << tk_shift) - 1) >> tk_shift;
+        for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o);
+        p.total += t;
+    }
+    p.total = uniform(p.total * rows);
+    p.waves = min(p.total, (int64_t)a.waves);
+    if (want < 0 && w >= p.waves) return p;
+    const int64_t goal = want < 0 ? kv_first_tile(w, p.total, p.waves) : 0;
+    int64_t ahead = 0;
+    for (int32_t b0 = 0; b0 < B; b0 += 64) {
+        int32_t mine = 0;
+        if (b0 + lane < B) mine = (int32_t)(((int64_t)seq_len(a, b0 + lane) + (1 << tk_shift) - 1) >> tk_shift);
+        int64_t incl = (int64_t)mine * rows;
+        for (int o = 1; o < 64; o <<= 1) {
+            const int64_t up = __shfl_up(incl, o);
+            if (lane >= o) incl += up;
         }
-        red[tid] = s;
-        __syncthreads();
-        for (int w = 128; w > 0; w >>= 1) {
-            if (tid < w) red[tid] = (red[tid] >= red[tid + w] || red[tid + w] != red[tid + w]) ? red[tid] : red[tid + w];
-            __syncthreads();
+        const bool here = want < 0 ? ahead + incl > goal : b0 + lane == want;
+        const uint64_t hit = __ballot(here);
+        if (hit) {
+            const int l = __builtin_ctzll(hit);
+            p.b = b0 + l;
+            p.tiles = __builtin_amdgcn_readlane(mine, l);
+            p.first = uniform(ahead + __shfl(incl, l)) - (int64_t)p.tiles * rows;
+            return p;
         }
-        const float mn = fmaxf(m, red[0]), base = mn == -INFINITY ? 0.f : mn;
-        p[tid] = vrow[tid] ? exp2f(s - base) : 0.f;
-        const float f = exp2f(m - base);
-        m = mn;
-        l *= f;
-        acc *= f;
-        __syncthreads();
-        for (int i = 0; i < 256; ++i) {
-            if (!vrow[i]) continue;
-            l += p[i];
-            if (tid < hd) acc = fmaf(p[i], P::get(vrow[i][tid]), acc);
+        ahead += uniform(__shfl(incl, 63));
+    }
+    return p;
+}
+
+template <int DT, bool F8, int HDP, bool PAD>
+struct Walk {
+    typedef Mma<DT> M;
+    static constexpr int NC = HDP / 32;                             // 32-element pieces of a row
+    static constexpr int DL = HDP >= 128 ? 8 : HDP / 16;            // value elements of a lane, per block of 16 lanes
+    static constexpr int VB = HDP > 128 ? HDP / 128 : 1;            // such blocks in a row
+    static constexpr int NT = F8 ? (HDP >= 256 ? 1 : HDP == 128 ? 2 : 4) : (HDP >= 128 ? 1 : HDP == 64 ? 2 : 4);
+    static constexpr int TK = 32 * NT, TK_SHIFT = NT == 1 ? 5 : NT == 2 ? 6 : 7;
+    static constexpr bool K16 = F8 && !PAD && HDP >= 64;            // e4m3 keys in 16-byte loads
+    static constexpr int KW = F8 ? 2 : 4, VW = F8 ? (DL >= 4 ? DL / 4 : 1) : DL / 2;   // dwords of a key / value piece
+    static constexpr int ES = F8 ? 1 : 2;
+
+    const AttnArgs& a;
+    int lane, r, j;                         // lane, lane % 16, lane / 16
+    int32_t n;                              // positions of the sequence
+    const int32_t* table;
+    int32_t ent, ent0;                      // 64 entries of the table row, one a lane, from entry ent0 on
+    const char *kbase, *vbase;              // key head's part of the pages
+    uint32_t koff, voff;                    // lane's bytes in a 16-key piece
+    uint32_t kmask;                         // PAD: bit c: piece c of this lane is inside the row
+    u32x4 q[NC];
+    uint32_t kr[NT][2][NC][KW], vr[NT][8][VB][VW];
+    f32x4 o[VB * DL];
+    float m, l, kscale;
+    uint32_t ok;                            // pieces of the tile in the registers whose page is there
+    bool full;                              // every position of that tile counts
+
+    __device__ __forceinline__ Walk(const AttnArgs& args) : a(args) {
+        lane = lane_id();
+        r = lane & 15;
+        j = lane >> 4;
+    }
+
+    __device__ __forceinline__ void begin(int32_t b, int32_t kh, int32_t qt, int32_t len) {
+        n = len;
+        table = a.kv.table + b * a.kv.table_stride;
+        ent0 = -64;
+        kbase = a.kv.k.ptr + kh * a.kv.k.head_stride;
+        vbase = a.kv.v.ptr + kh * a.kv.v.head_stride;
+        const int hd = a.kv.head_dim;
+        koff = r * (uint32_t)a.kv.k.slot_stride;
+        if (!PAD) koff += (K16 ? 16 : 8 * ES) * j;
+        const int vd = VB > 1 ? 8 * r : DL * r;
+        voff = 4 * j * (uint32_t)a.kv.v.slot_stride + (!PAD || vd < hd ? vd * ES : 0);
+        kscale = a.scale * (a.kv.k.scale ? a.kv.k.scale[kh] : 1.f);
+        const int head = kh * a.group + qt * 16 + r;
+        const bool there = qt * 16 + r < a.group;
+        const char* qp = a.q + b * a.q_seq_stride + (int64_t)(there ? head : kh * a.group) * a.q_head_stride;
+        kmask = 0;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int d = K16 ? 64 * (c / 2) + 16 * j + 8 * (c % 2) : 32 * c + 8 * j;
+            const bool in = !PAD || d < hd;
+            kmask |= in ? 1u << c : 0;
+            const u32x4 w = *(const u32x4*)(qp + (in ? 2 * d : 0));
+            const u32x4 zero = {0, 0, 0, 0};
+            q[c] = there && in ? w : zero;
+        }
+#pragma unroll
+        for (int i = 0; i < VB * DL; ++i) o[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        m = -INFINITY;
+        l = 0.f;
+    }
+
+    // Base of 16-key piece s (wave-uniform); a piece whose page is not there points at page 0 and is left out later.
+    __device__ __forceinline__ int32_t page_of(int32_t key0) {
+        const int32_t e = key0 >> a.kv.page_shift;
+        if ((uint32_t)(e - ent0) >= 64u) {
+            ent0 = e;
+            const int64_t at = (int64_t)e + lane, last = ((int64_t)n - 1) >> a.kv.page_shift;
+            ent = at <= last ? table[at] : -1;
+        }
+        return kv_page_or_none(key0 < n ? __builtin_amdgcn_readlane(ent, e - ent0) : -1, a.kv.num_pages);
+    }
+
+    template <int W> static __device__ __forceinline__ void load(uint32_t (&to)[W], const char* p) {
+        if constexpr (W == 4) {
+            const u32x4 x = *(const u32x4*)p;
+            to[0] = x[0], to[1] = x[1], to[2] = x[2], to[3] = x[3];
+        } else if constexpr (W == 2) {
+            const u32x2 x = *(const u32x2*)p;
+            to[0] = x[0], to[1] = x[1];
+        } else if constexpr (F8 && DL == 2) {
+            to[0] = *(const uint16_t*)p;
+        } else {
+            to[0] = *(const uint32_t*)p;
         }
     }
-    if (tid < hd) {
-        const float vs = a.kv.v.scale ? a.kv.v.scale[kh] : 1.f;
-        ((raw*)a.out)[((int64_t)b * a.heads + h) * hd + tid] = E::put(l != 0.f ? acc / l * vs : 0.f);
+
+    int32_t pg[2 * NT];
+    __device__ __forceinline__ void pages(int32_t tile) {
+#pragma unroll
+        for (int s = 0; s < 2 * NT; ++s) pg[s] = page_of(tile * TK + 16 * s);
+    }
+    __device__ __forceinline__ void load_keys(int32_t tile) {
+#pragma unroll
+        for (int s = 0; s < 2 * NT; ++s) {
+            const int32_t slot = (tile * TK + 16 * s) & ((1 << a.kv.page_shift) - 1);
+            const char* base = kbase + (int64_t)max(pg[s], 0) * a.kv.k.page_stride + (int64_t)slot * a.kv.k.slot_stride;
+            if constexpr (K16) {
+#pragma unroll
+                for (int c = 0; c < NC / 2; ++c) {
+                    const u32x4 x = *(const u32x4*)(base + (koff + 64 * c));
+                    kr[s / 2][s % 2][2 * c][0] = x[0], kr[s / 2][s % 2][2 * c][1] = x[1];
+                    kr[s / 2][s % 2][2 * c + 1][0] = x[2], kr[s / 2][s % 2][2 * c + 1][1] = x[3];
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    const uint32_t d = PAD ? (kmask >> c & 1 ? (32 * c + 8 * j) * ES : 0) : 32 * c * ES;
+                    load<KW>(kr[s / 2][s % 2][c], base + (koff + d));
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void load_values(int32_t tile) {
+#pragma unroll
+        for (int s = 0; s < 2 * NT; ++s) {
+            const int32_t slot = (tile * TK + 16 * s) & ((1 << a.kv.page_shift) - 1);
+            const char* base = vbase + (int64_t)max(pg[s], 0) * a.kv.v.page_stride + (int64_t)slot * a.kv.v.slot_stride;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int b = 0; b < VB; ++b) {
+                    const uint32_t d = PAD && VB > 1 ? (8 * r + 128 * b < a.kv.head_dim ? 128 * b * ES : 0) : 128 * b * ES;
+                    load<VW>(vr[s / 2][4 * (s % 2) + i][b], base + (int64_t)i * a.kv.v.slot_stride + (voff + d));
+                }
+        }
+    }
+    __device__ __forceinline__ void note(int32_t tile) {
+        ok = 0;
+#pragma unroll
+        for (int s = 0; s < 2 * NT; ++s) ok |= pg[s] >= 0 ? 1u << s : 0;
+        full = ok == (1u << (2 * NT)) - 1 && (tile + 1) * TK <= n;
+    }
+
+    // Keys of one piece as the 8 elements of each 32-element step.
+    __device__ __forceinline__ u32x4 key_step(const uint32_t (&w)[KW], int c) const {
+        u32x4 x;
+        if constexpr (F8) {
+            x[0] = M::template from_f8<false>(w[0]), x[1] = M::template from_f8<true>(w[0]);
+            x[2] = M::template from_f8<false>(w[1]), x[3] = M::template from_f8<true>(w[1]);
+        } else {
+            x[0] = w[0], x[1] = w[1], x[2] = w[2], x[3] = w[3];
+        }
+        if (PAD) {
+            const u32x4 zero = {0, 0, 0, 0};
+            x = kmask >> c & 1 ? x : zero;
+        }
+        return x;
+    }
+
+    // Tiles [t0, t1) of the row set by begin().
+    __device__ __forceinline__ void run(int32_t t0, int32_t t1) {
+        pages(t0);
+        load_keys(t0);
+        load_values(t0);
+        for (int32_t t = t0; t < t1; ++t) {
+            note(t);
+            const int32_t tn = min(t + 1, t1 - 1);      // the last step loads its own tile once more
+            f32x4 s[2 * NT];
+#pragma unroll
+            for (int i = 0; i < 2 * NT; ++i) {
+                s[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < NC; ++c) s[i] = M::dot(key_step(kr[i / 2][i % 2][c], c), q[c], s[i]);
+            }
+            pages(tn);
+            load_keys(tn);
+            float top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 2 * NT; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[i][e] *= kscale;
+            if (!full) {
+#pragma unroll
+                for (int i = 0; i < 2 * NT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const bool in = (ok >> i & 1) && t * TK + 16 * i + 4 * j + e < n;
+                        s[i][e] = in ? s[i][e] : -INFINITY;
+#pragma unroll
+                        for (int b = 0; b < VB; ++b)
+#pragma unroll
+                            for (int w = 0; w < VW; ++w) vr[i / 2][4 * (i % 2) + e][b][w] = in ? vr[i / 2][4 * (i % 2) + e][b][w] : 0;
+                    }
+            }
+#pragma unroll
+            for (int i = 0; i < 2 * NT; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top = fmaxf(top, s[i][e]);
+            if (__any(top > m + LAZY)) {                // the maximum moves for all heads of the tile at once
+                const float mn = fmaxf(m, max_over_keys(top)), f = exp2f(m - (mn == -INFINITY ? 0.f : mn));
+                m = mn;
+                l *= f;
+                const f32x4 g = {__shfl(f, 4 * j), __shfl(f, 4 * j + 1), __shfl(f, 4 * j + 2), __shfl(f, 4 * j + 3)};
+#pragma unroll
+                for (int i = 0; i < VB * DL; ++i) o[i] *= g;
+            }
+            const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+            for (int i = 0; i < 2 * NT; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[i][e] = exp2f(s[i][e] - base);
+                    l += s[i][e];
+                }
+#pragma unroll
+            for (int g = 0; g < NT; ++g) {
+                u32x4 ph, pl;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float x = s[2 * g + e / 2][2 * (e % 2)], y = s[2 * g + e / 2][2 * (e % 2) + 1];
+                    uint32_t head, rest;
+                    M::split(x, y, head, rest);
+                    ph[e] = head;
+                    pl[e] = rest;
+                }
+#pragma unroll
+                for (int b = 0; b < VB; ++b)
+#pragma unroll
+                    for (int i = 0; i < DL; ++i) {
+                        u32x4 x;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            if constexpr (F8) {
+                                const uint32_t w = __builtin_amdgcn_perm(vr[g][2 * e + 1][b][i / 4], vr[g][2 * e][b][i / 4],
+                                                                         i % 4 < 2 ? 0x05010400u : 0x07030602u);
+                                x[e] = i % 2 ? M::template from_f8<true>(w) : M::template from_f8<false>(w);
+                            } else {
+                                x[e] = __builtin_amdgcn_perm(vr[g][2 * e + 1][b][i / 2], vr[g][2 * e][b][i / 2],
+                                                             i % 2 ? 0x07060302u : 0x05040100u);
+                            }
+                        }
+                        o[b * DL + i] = M::dot(ph, x, o[b * DL + i]);
+                        o[b * DL + i] = M::dot(pl, x, o[b * DL + i]);
+                    }
+            }
+            load_values(tn);
+        }
+    }
+
+    // The finished row: every head of the tile divided by its sum, rounded and stored.
+    __device__ __forceinline__ void store(int32_t b, int32_t kh, int32_t qt) {
+        typedef KvElem<DT> E;
+        const float sum = sum_over_keys(l), vs = a.kv.v.scale ? a.kv.v.scale[kh] : 1.f;
+        const float inv = sum != 0.f ? vs / sum : 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int row = 4 * j + e;
+            const float f = __shfl(inv, row);
+            if (qt * 16 + row >= a.group) continue;
+            char* y = a.out + ((int64_t)b * a.heads + kh * a.group + qt * 16 + row) * a.kv.head_dim * 2;
+#pragma unroll
+            for (int v = 0; v < VB; ++v) {
+                const int d = VB > 1 ? 8 * r + 128 * v : DL * r;
+                if (PAD && d >= a.kv.head_dim) continue;
+                uint32_t w[DL / 2];
+#pragma unroll
+                for (int i = 0; i < DL / 2; ++i) w[i] = M::pack(o[v * DL + 2 * i][e] * f, o[v * DL + 2 * i + 1][e] * f);
+                if constexpr (DL == 8) *(u32x4*)(y + 2 * d) = (u32x4){w[0], w[1], w[2], w[3]};
+                else if constexpr (DL == 4) *(u32x2*)(y + 2 * d) = (u32x2){w[0], w[1]};
+                else *(uint32_t*)(y + 2 * d) = w[0];
+            }
+        }
+    }
+
+    // A part of a row, for the join: unnormalised sums, maximum and sum of the weights.
+    __device__ __forceinline__ void store_part(int64_t slot, int32_t qt) {
+        const int rows = min(a.group, 16);
+        const float sum = sum_over_keys(l);
+        if (j == 0 && qt * 16 + r < a.group) {
+            float* ml = a.part_ml + (slot * rows + r) * 2;
+            ml[0] = m;
+            ml[1] = sum;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int row = 4 * j + e;
+            if (qt * 16 + row >= a.group) continue;
+            float* y = a.part_o + (slot * rows + row) * HDP;
+#pragma unroll
+            for (int v = 0; v < VB; ++v)
+#pragma unroll
+                for (int i = 0; i < DL; ++i) y[(VB > 1 ? 8 * r + 128 * v : DL * r) + i] = o[v * DL + i][e];
+        }
+    }
+};
+
+// The tiles of all (sequence, key head, query tile) rows in one line, cut into equal runs, one per wavefront: lengths are
+// on the device, and this is even for any of them.  A row inside one run is finished here; the first and the last row
+// of a run may be parts (slots 2w and 2w + 1).
+template <int DT, bool F8, int HDP, bool PAD>
+__global__ void __launch_bounds__(64 * WAVES, HDP > 128 ? 1 : 2) attn_walk_kernel(AttnArgs a) {
+    typedef Walk<DT, F8, HDP, PAD> W;
+    // few tiles are spread over all blocks: the first wavefronts of all blocks come first
+    const int64_t w = (int64_t)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * gridDim.x + blockIdx.x;
+    const int32_t rows = a.kv.kv_heads * a.qtiles;
+    Place p = find_place(a, W::TK_SHIFT, rows, w, -1);
+    if (w >= p.waves) return;
+    int64_t t = kv_first_tile(w, p.total, p.waves);
+    const int64_t end = kv_first_tile(w + 1, p.total, p.waves);
+    int32_t row = (int32_t)((t - p.first) / p.tiles), b = p.b, tiles = p.tiles;
+    int32_t from = (int32_t)(t - p.first - (int64_t)row * tiles);
+    W walk(a);
+    while (true) {
+        const int32_t kh = row / a.qtiles, qt = row % a.qtiles;
+        const int32_t to = (int32_t)min((int64_t)tiles, from + (end - t));
+        walk.begin(b, kh, qt, seq_len(a, b));
+        walk.run(from, to);
+        if (from == 0 && to == tiles) walk.store(b, kh, qt);
+        else walk.store_part(2 * w + (from == 0), qt);
+        t += to - from;
+        if (t >= end) return;
+        from = 0;
+        if (++row == rows) {
+            row = 0;
+            do {
+                ++b;
+                tiles = (seq_len(a, b) + W::TK - 1) >> W::TK_SHIFT;
+            } while (tiles == 0);       // t < end <= total: a later sequence has tiles
+        }
+    }
+}
+
+// Rows that lie in several runs: the parts of head `row` weighted by 2^(m - max) and added in the order of the runs.
+// Sequences without a position get zeros here.
+template <int DT, int HDP>
+__global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int tk_shift) {
+    __shared__ float acc[4][HDP], tot[4];
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    const int32_t b = blockIdx.x / a.heads, head = blockIdx.x % a.heads, kh = head / a.group, in = head % a.group;
+    const int32_t row = kh * a.qtiles + in / 16, hd = a.kv.head_dim, gr = min(a.group, 16);
+    const Place p = find_place(a, tk_shift, a.kv.kv_heads * a.qtiles, 0, b);
+    typedef KvElem<DT> E;
+    typename E::raw* y = (typename E::raw*)a.out + ((int64_t)b * a.heads + head) * hd;
+    if (p.tiles == 0) {
+        for (int d = tid; d < hd; d += 256) y[d] = 0;
+        return;
+    }
+    const int64_t first = p.first + (int64_t)row * p.tiles;
+    const int64_t w0 = kv_wave_of_tile(first, p.total, p.waves), w1 = kv_wave_of_tile(first + p.tiles - 1, p.total, p.waves);
+    if (w0 == w1) return;
+    float top = -INFINITY;
+    for (int64_t w = w0 + lane; w <= w1; w += 64) top = fmaxf(top, a.part_ml[((2 * w + (w == w0)) * gr + in % 16) * 2]);
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    const float base = top == -INFINITY ? 0.f : top;
+    constexpr int PER = HDP >= 64 ? HDP / 64 : 1;
+    float sum = 0.f, x[PER] = {};
+    for (int64_t w = w0 + wv; w <= w1; w += 4) {
+        const int64_t slot = (2 * w + (w == w0)) * gr + in % 16;
+        const float f = exp2f(a.part_ml[slot * 2] - base);
+        sum += f * a.part_ml[slot * 2 + 1];
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            if (HDP >= 64 || lane < HDP) x[i] += f * a.part_o[slot * HDP + lane + 64 * i];
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+        if (HDP >= 64 || lane < HDP) acc[wv][lane + 64 * i] = x[i];
+    if (lane == 0) tot[wv] = sum;
+    __syncthreads();
+    const float s = (tot[0] + tot[1]) + (tot[2] + tot[3]), vs = a.kv.v.scale ? a.kv.v.scale[kh] : 1.f;
+    const float inv = s != 0.f ? vs / s : 0.f;
+    if (tid < hd) y[tid] = E::put(((acc[0][tid] + acc[1][tid]) + (acc[2][tid] + acc[3][tid])) * inv);
+}
+
+int padded(int64_t hd) { return hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
+
+int waves_for(int64_t hd) { return hd > 128 ? 1024 : 2048; }
+
+template <int DT, bool F8, int HDP, bool PAD>
+void launch(const AttnArgs& a, hipStream_t s) {
+    hipLaunchKernelGGL((attn_walk_kernel<DT, F8, HDP, PAD>), dim3(a.waves / WAVES), dim3(64 * WAVES), 0, s, a);
+    hipLaunchKernelGGL((attn_join_kernel<DT, HDP>), dim3((unsigned)a.kv.sequences * a.heads), dim3(256), 0, s, a,
+                       Walk<DT, F8, HDP, PAD>::TK_SHIFT);
+}
+
+template <int DT, bool F8>
+void launch_dim(const AttnArgs& a, bool pad, hipStream_t s) {
+    switch (padded(a.kv.head_dim)) {
+        case 32: return pad ? launch<DT, F8, 32, true>(a, s) : launch<DT, F8, 32, false>(a, s);
+        case 64: return pad ? launch<DT, F8, 64, true>(a, s) : launch<DT, F8, 64, false>(a, s);
+        case 128: return pad ? launch<DT, F8, 128, true>(a, s) : launch<DT, F8, 128, false>(a, s);
+        default: return pad ? launch<DT, F8, 256, true>(a, s) : launch<DT, F8, 256, false>(a, s);
     }
 }
 
 }  // namespace
 
 extern "C" int64_t hyena_attn_step_ws_bytes(int64_t sequences, int64_t heads, int64_t kv_heads, int64_t head_dim) {
-    (void)sequences, (void)heads, (void)kv_heads, (void)head_dim;
-    return 0;
+    if (sequences <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || head_dim > 256 || heads % kv_heads) return 0;
+    const int64_t g = heads / kv_heads, rows = g < 16 ? g : 16;
+    return 2 * (int64_t)waves_for(head_dim) * rows * (padded(head_dim) + 2) * 4;
 }
 
 extern "C" int hyena_attn_step(const hyena_kv_pages* kv, const hyena_heads* q, const int32_t* lens, float scale, void* out,
@@ -90,8 +545,9 @@ extern "C" int hyena_attn_step(const hyena_kv_pages* kv, const hyena_heads* q, c
     if (kv->sequences * heads >= (1LL << 31))
         return hyena_fail(HYENA_EINVAL, "%s: %lld sequences of %lld heads", who, (long long)kv->sequences, (long long)heads);
     const int64_t need = hyena_attn_step_ws_bytes(kv->sequences, heads, kv->kv_heads, kv->head_dim);
-    if (need > 0 && (!ws || ws_bytes < need))
-        return hyena_fail(HYENA_EINVAL, "%s: workspace of %lld bytes, %lld needed", who, (long long)ws_bytes, (long long)need);
+    if (!ws || ws_bytes < need || ((uintptr_t)ws & 15))
+        return hyena_fail(HYENA_EINVAL, "%s: workspace of %lld bytes (16-byte aligned), %lld needed", who, (long long)ws_bytes,
+                          (long long)need);
     a.q = (const char*)q->ptr;
     a.q_seq_stride = q->token_stride * 2;
     a.q_head_stride = q->head_stride * 2;
@@ -100,14 +556,17 @@ extern "C" int hyena_attn_step(const hyena_kv_pages* kv, const hyena_heads* q, c
     a.scale = scale * 1.4426950408889634f;
     a.heads = (int32_t)heads;
     a.group = (int32_t)(heads / kv->kv_heads);
+    a.qtiles = (a.group + 15) / 16;
+    a.waves = waves_for(kv->head_dim);
+    a.part_o = (float*)ws;
+    a.part_ml = a.part_o + 2 * (int64_t)a.waves * (a.group < 16 ? a.group : 16) * padded(kv->head_dim);
+    const bool f8 = kv->dtype == HYENA_DTYPE_F8E4M3;
+    // the plain form loads 16 bytes of a row at a time and whole rows; other row lengths and, in 8 bits, strides that
+    // are only 8-byte multiples take the form that masks the pieces behind a row's end
+    const bool pad = kv->head_dim != padded(kv->head_dim) ||
+                     (f8 && ((kv->k.page_stride | kv->k.head_stride | kv->k.slot_stride) & 15));
     hipStream_t s = (hipStream_t)stream;
-    const dim3 grid((unsigned)(kv->sequences * heads));
-#define AT_CASE(D, P)                                                                            \
-    if (dtype == D && kv->dtype == P) hipLaunchKernelGGL((attn_step_kernel<D, P>), grid, dim3(256), 0, s, a);
-    AT_CASE(HYENA_DTYPE_BF16, HYENA_DTYPE_BF16)
-    AT_CASE(HYENA_DTYPE_F16, HYENA_DTYPE_F16)
-    AT_CASE(HYENA_DTYPE_BF16, HYENA_DTYPE_F8E4M3)
-    AT_CASE(HYENA_DTYPE_F16, HYENA_DTYPE_F8E4M3)
-#undef AT_CASE
+    if (dtype == HYENA_DTYPE_BF16) f8 ? launch_dim<HYENA_DTYPE_BF16, true>(a, pad, s) : launch_dim<HYENA_DTYPE_BF16, false>(a, pad, s);
+    else f8 ? launch_dim<HYENA_DTYPE_F16, true>(a, pad, s) : launch_dim<HYENA_DTYPE_F16, false>(a, pad, s);
     return hyena_check_launch(who);
 }

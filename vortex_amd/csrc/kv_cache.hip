@@ -8,7 +8,7 @@ int kv_pages_check(const hyena_kv_pages* kv, int dtype, KvPages* out, const char
         return hyena_fail(HYENA_ENOSUP, "%s: activations of type %d (bfloat16 and float16 have kernels)", who, dtype);
     if (kv->dtype != dtype && kv->dtype != HYENA_DTYPE_F8E4M3)
         return hyena_fail(HYENA_ENOSUP, "%s: pages of type %d with activations of type %d", who, kv->dtype, dtype);
-    if (kv->num_pages < 0 || kv->num_pages >= (1LL << 31) || kv->kv_heads <= 0 || kv->kv_heads > 65535 || kv->sequences < 0 ||
+    if (kv->num_pages <= 0 || kv->num_pages >= (1LL << 31) || kv->kv_heads <= 0 || kv->kv_heads > 65535 || kv->sequences < 0 ||
         kv->sequences >= (1LL << 31) || kv->table_width < 0 || kv->table_width >= (1LL << 31) || kv->head_dim <= 0)
         return hyena_fail(HYENA_EINVAL, "%s: bad sizes pages=%lld kv_heads=%lld sequences=%lld table_width=%lld head_dim=%lld", who,
                           (long long)kv->num_pages, (long long)kv->kv_heads, (long long)kv->sequences,
