@@ -457,7 +457,8 @@ int hyena_fir_layer_fwd(const hyena_proj_fwd* proj,
  * A page id outside 0..num_pages-1 names no page: nothing is read from or written to it (attention leaves its positions
  * out, an append drops them), and so do positions beyond table_width*page_size.
  * Rules (others: HYENA_ENOSUP / HYENA_EALIGN): head_dim a multiple of 8 up to 256; page_size a power of two from 16 to
- * 65536; strides multiples of 8 elements, pointers 16-byte aligned. */
+ * 65536; strides multiples of 8 elements (that of a dimension of one element is not looked at), pointers 16-byte
+ * aligned. */
 typedef struct hyena_kv_side {
     void* ptr;
     int64_t page_stride, head_stride, slot_stride;
@@ -486,9 +487,9 @@ typedef struct hyena_heads {
  * q [sequences][heads][head_dim] (token_stride = sequence stride), out the same, contiguous, of the type of q (`dtype`:
  * BF16 or F16).  lens[s] <= 0 gives zeros; lens[s] beyond the table's reach counts as its reach.  Values behind
  * lens[s] in a page may be anything, NaN included.  Sums and softmax statistics are float32.
- * ws: hyena_attn_step_ws_bytes(sequences, heads, kv_heads, head_dim) bytes of device memory for the parts of long
+ * ws: hyena_attn_step_ws_bytes(kv, heads) bytes of device memory (16-byte aligned; may be 0) for the parts of long
  * sequences, contents of no interest before and after; calls that overlap in time need one each. */
-int64_t hyena_attn_step_ws_bytes(int64_t sequences, int64_t heads, int64_t kv_heads, int64_t head_dim);
+int64_t hyena_attn_step_ws_bytes(const hyena_kv_pages* kv, int64_t heads);
 int hyena_attn_step(const hyena_kv_pages* kv, const hyena_heads* q, const int32_t* lens, float scale, void* out,
                     void* ws, int64_t ws_bytes, int64_t heads, int dtype, void* stream);
 

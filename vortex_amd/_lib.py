@@ -55,29 +55,6 @@ class ProjFwd(Structure):
                 ("gate_stride", c_int64), ("ch_stride", c_int64)]
 
 
-class KvSide(Structure):
-    """hyena_kv_side: the pages of the keys or of the values."""
-    _fields_ = [("ptr", c_void_p), ("page_stride", c_int64), ("head_stride", c_int64), ("slot_stride", c_int64),
-                ("scale", c_void_p)]
-
-
-class KvPages(Structure):
-    """hyena_kv_pages: one layer's paged key / value cache and the page table of the sequences."""
-    _fields_ = [("k", KvSide), ("v", KvSide), ("num_pages", c_int64), ("page_size", c_int64), ("kv_heads", c_int64),
-                ("head_dim", c_int64), ("table", c_void_p), ("table_stride", c_int64), ("table_width", c_int64),
-                ("sequences", c_int64), ("dtype", c_int), ("reserved", c_int)]
-
-
-class HeadRows(Structure):
-    """hyena_heads: token rows [tokens][heads][head_dim]."""
-    _fields_ = [("ptr", c_void_p), ("token_stride", c_int64), ("head_stride", c_int64)]
-
-
-class KvPools(Structure):
-    """hyena_kv_pools: pools of pages of one size."""
-    _fields_ = [("base", c_void_p), ("pool_stride", c_int64), ("page_stride", c_int64), ("pages", c_int64)]
-
-
 _lib = None
 
 
@@ -150,12 +127,13 @@ def lib():
     L.hyena_featurizer_gates_fwd.argtypes = [POINTER(ProjFwd), c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p]
     L.hyena_fir_layer_fwd.argtypes = [POINTER(ProjFwd), c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int64,
                                       c_int64, c_int64, c_int64, c_int64, c_int, c_void_p]
-    KV, HR, KP = POINTER(KvPages), POINTER(HeadRows), POINTER(KvPools)
-    L.hyena_attn_step_ws_bytes.argtypes = [c_int64, c_int64, c_int64, c_int64]
-    L.hyena_attn_step.argtypes = [KV, HR, c_void_p, c_float, c_void_p, c_void_p, c_int64, c_int64, c_int, c_void_p]
-    L.hyena_rotary_append.argtypes = [KV, HR, HR, HR, HR, HR, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int64,
+    # the paged-cache calls take their structures as packed bytes (kv_cache.py)
+    kv, hr, kp = c_char_p, c_char_p, c_char_p
+    L.hyena_attn_step_ws_bytes.argtypes = [kv, c_int64]
+    L.hyena_attn_step.argtypes = [kv, hr, c_void_p, c_float, c_void_p, c_void_p, c_int64, c_int64, c_int, c_void_p]
+    L.hyena_rotary_append.argtypes = [kv, hr, hr, hr, hr, hr, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int64,
                                       c_int64, c_int, c_void_p]
-    L.hyena_kv_copy_pages.argtypes = [KP, KP, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_void_p]
+    L.hyena_kv_copy_pages.argtypes = [kp, kp, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_void_p]
     for name in EXPORTS:
         fn = getattr(L, name)
         if name not in ("hyena_version", "hyena_last_error_string"):

@@ -524,10 +524,11 @@ void launch_dim(const AttnArgs& a, bool pad, hipStream_t s) {
 
 }  // namespace
 
-extern "C" int64_t hyena_attn_step_ws_bytes(int64_t sequences, int64_t heads, int64_t kv_heads, int64_t head_dim) {
-    if (sequences <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || head_dim > 256 || heads % kv_heads) return 0;
-    const int64_t g = heads / kv_heads, rows = g < 16 ? g : 16;
-    return 2 * (int64_t)waves_for(head_dim) * rows * (padded(head_dim) + 2) * 4;
+extern "C" int64_t hyena_attn_step_ws_bytes(const hyena_kv_pages* kv, int64_t heads) {
+    if (!kv || kv->sequences <= 0 || heads <= 0 || kv->kv_heads <= 0 || kv->head_dim <= 0 || kv->head_dim > 256 || heads % kv->kv_heads)
+        return 0;
+    const int64_t g = heads / kv->kv_heads, rows = g < 16 ? g : 16;
+    return 2 * (int64_t)waves_for(kv->head_dim) * rows * (padded(kv->head_dim) + 2) * 4;
 }
 
 extern "C" int hyena_attn_step(const hyena_kv_pages* kv, const hyena_heads* q, const int32_t* lens, float scale, void* out,
@@ -540,17 +541,18 @@ extern "C" int hyena_attn_step(const hyena_kv_pages* kv, const hyena_heads* q, c
         return hyena_fail(HYENA_EINVAL, "%s: %lld heads over %lld key heads", who, (long long)heads, (long long)kv->kv_heads);
     if (kv->sequences == 0) return 0;
     if (!q || !q->ptr || !lens || !out) return hyena_fail(HYENA_EINVAL, "%s: q, lens and out are required", who);
-    if (((uintptr_t)q->ptr & 15) || ((uintptr_t)out & 15) || q->token_stride % 8 || q->head_stride % 8)
-        return hyena_fail(HYENA_EALIGN, "%s: q and out must be 16-byte aligned with strides of a multiple of 8 elements", who);
+    if (((uintptr_t)out & 15)) return hyena_fail(HYENA_EALIGN, "%s: out must be 16-byte aligned", who);
+    KvHeads qh;
+    if ((rc = kv_heads_check(q, true, "q", kv->sequences, heads, &qh, who))) return rc;
     if (kv->sequences * heads >= (1LL << 31))
         return hyena_fail(HYENA_EINVAL, "%s: %lld sequences of %lld heads", who, (long long)kv->sequences, (long long)heads);
-    const int64_t need = hyena_attn_step_ws_bytes(kv->sequences, heads, kv->kv_heads, kv->head_dim);
+    const int64_t need = hyena_attn_step_ws_bytes(kv, heads);
     if (!ws || ws_bytes < need || ((uintptr_t)ws & 15))
         return hyena_fail(HYENA_EINVAL, "%s: workspace of %lld bytes (16-byte aligned), %lld needed", who, (long long)ws_bytes,
                           (long long)need);
-    a.q = (const char*)q->ptr;
-    a.q_seq_stride = q->token_stride * 2;
-    a.q_head_stride = q->head_stride * 2;
+    a.q = qh.ptr;
+    a.q_seq_stride = qh.token_stride;
+    a.q_head_stride = qh.head_stride;
     a.lens = lens;
     a.out = (char*)out;
     a.scale = scale * 1.4426950408889634f;

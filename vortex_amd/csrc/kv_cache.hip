@@ -1,4 +1,7 @@
 // Paged key / value cache: rotary positions with the append, and page copies.
+#include <algorithm>
+
+#include "kv_addr.h"
 #include "kv_cache.h"
 
 int kv_pages_check(const hyena_kv_pages* kv, int dtype, KvPages* out, const char* who) {
@@ -21,7 +24,9 @@ int kv_pages_check(const hyena_kv_pages* kv, int dtype, KvPages* out, const char
     const hyena_kv_side* in[2] = {&kv->k, &kv->v};
     KvSide* to[2] = {&out->k, &out->v};
     for (int i = 0; i < 2; ++i) {
-        const hyena_kv_side& s = *in[i];
+        hyena_kv_side s = *in[i];
+        if (kv->num_pages == 1) s.page_stride = 0;
+        if (kv->kv_heads == 1) s.head_stride = 0;
         if (((uintptr_t)s.ptr & 15) || s.page_stride % 8 || s.head_stride % 8 || s.slot_stride % 8)
             return hyena_fail(HYENA_EALIGN, "%s: pages must be 16-byte aligned with strides of a multiple of 8 elements", who);
         *to[i] = {(char*)s.ptr, s.page_stride * es, s.head_stride * es, s.slot_stride * es, s.scale};
@@ -37,94 +42,257 @@ int kv_pages_check(const hyena_kv_pages* kv, int dtype, KvPages* out, const char
     return 0;
 }
 
+int kv_heads_check(const hyena_heads* h, bool required, const char* name, int64_t tokens, int64_t heads, KvHeads* out,
+                   const char* who) {
+    *out = {nullptr, 0, 0};
+    if (!h || !h->ptr) return required ? hyena_fail(HYENA_EINVAL, "%s: %s is required", who, name) : 0;
+    const int64_t ts = tokens == 1 ? 0 : h->token_stride, hs = heads == 1 ? 0 : h->head_stride;
+    if (((uintptr_t)h->ptr & 15) || ts % 8 || hs % 8)
+        return hyena_fail(HYENA_EALIGN, "%s: %s must be 16-byte aligned with strides of a multiple of 8 elements", who, name);
+    *out = {(char*)h->ptr, ts * 2, hs * 2};
+    return 0;
+}
+
 namespace {
 
-struct Heads {
-    char* ptr;
-    int64_t token_stride, head_stride;      // bytes
+struct Role {                               // the rows of q, k or v in a block's work
+    KvHeads src, dst;                       // dst.ptr NULL: no rows of activations are written
+    uint32_t heads, magic;                  // magic = ceil(2^32 / heads): i / heads = (i * magic) >> 32 for i * heads < 2^32
 };
 
 struct AppendArgs {
     KvPages kv;
-    Heads q, k, v, q_out, k_out;
+    Role role[3];                           // q, k, v
     const int32_t *pos, *seq;
     const double* turns;
-    int32_t heads, half, per_seq;           // half = rotary_dim / 2
-    int32_t interleaved, zero_skipped;
+    int64_t tokens;
+    int32_t half, per_seq, zero_skipped;    // half = rotary_dim / 2
+    int32_t block_tokens, block_rounds;     // what a block takes: tokens, and rounds over their heads
 };
 
-// One block per token; a thread takes pairs (rotated part) and single elements (the rest) of every head in turn.
-template <int DT, int KVDT>
-__global__ void __launch_bounds__(256) rotary_append_kernel(AppendArgs a) {
+constexpr int APPEND_THREADS = 256;
+constexpr int APPEND_TOKENS = 16;           // of a block at most: 16 * 128 pairs fill the LDS tables
+constexpr int BATCH = 4;                    // pieces a thread has in flight
+
+// VEC elements of an activation row as float32, and back.
+template <int DT, int VEC> struct Piece {
     typedef KvElem<DT> E;
-    typedef KvElem<KVDT> P;
-    typedef typename E::raw raw;
-    typedef typename P::raw praw;
-    const int64_t t = blockIdx.x;
-    const int64_t pos = a.pos[t];
-    const int hd = a.kv.head_dim, K = a.kv.kv_heads, half = a.half;
-    if (pos < 0 && !a.zero_skipped) return;
-    const int64_t s = a.seq ? a.seq[t] : t / a.per_seq;
-    int64_t page = -1;
-    if (pos >= 0 && s >= 0 && s < a.kv.sequences && pos < a.kv.reach) {
-        page = a.kv.table[s * a.kv.table_stride + (pos >> a.kv.page_shift)];
-        if (page >= a.kv.num_pages) page = -1;
+    static constexpr int W = VEC >= 2 ? VEC / 2 : 1;
+    uint32_t w[W];
+    __device__ __forceinline__ void load(const char* p) {
+        if constexpr (VEC == 8) {
+            const u32x4 x = *(const u32x4*)p;
+            w[0] = x[0], w[1] = x[1], w[2] = x[2], w[3] = x[3];
+        } else if constexpr (VEC == 2) w[0] = *(const uint32_t*)p;
+        else w[0] = *(const uint16_t*)p;
     }
-    const int64_t slot = pos & ((1LL << a.kv.page_shift) - 1);
-    const int units = half + (hd - 2 * half);                // pairs, then single elements
-    for (int w = threadIdx.x; w < units * (a.heads + 2 * K); w += 256) {
-        const int hh = w / units, u = w % units;
-        const bool is_q = hh < a.heads, is_v = hh >= a.heads + K;
-        const int h = is_q ? hh : (is_v ? hh - a.heads - K : hh - a.heads);
-        const Heads& src = is_q ? a.q : (is_v ? a.v : a.k);
-        const raw* x = (const raw*)(src.ptr + t * src.token_stride + h * src.head_stride);
-        const bool pair = u < half;
-        const int i0 = pair ? (a.interleaved ? 2 * u : u) : half + u, i1 = a.interleaved ? 2 * u + 1 : u + half;
-        float y0 = E::get(x[i0]), y1 = pair ? E::get(x[i1]) : 0.f;
-        if (pair && !is_v) {
-            const double turn = (double)pos * a.turns[u];
-            float sn, cs;
-            sincospif(2.f * (float)(turn - rint(turn)), &sn, &cs);
-            const float x0 = y0, x1 = y1;
-            y0 = x0 * cs - x1 * sn;
-            y1 = x0 * sn + x1 * cs;
+    __device__ __forceinline__ void get(float (&x)[VEC]) const {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) x[i] = i % 2 ? E::hi(w[i / 2]) : E::lo(w[i / 2]);
+    }
+    static __device__ __forceinline__ void put(char* p, const float (&x)[VEC]) {
+        uint32_t o[W];
+#pragma unroll
+        for (int i = 0; i < W; ++i) o[i] = E::pack(x[2 * i], x[(2 * i + 1) % VEC]);
+        if constexpr (VEC == 8) *(u32x4*)p = (u32x4){o[0], o[1], o[2], o[3]};
+        else if constexpr (VEC == 2) *(uint32_t*)p = o[0];
+        else *(uint16_t*)p = (uint16_t)o[0];
+    }
+    static __device__ __forceinline__ void put_f8(char* p, const float (&x)[VEC], float scale) {
+        typedef KvElem<HYENA_DTYPE_F8E4M3> P;
+        uint32_t o[W];
+#pragma unroll
+        for (int i = 0; i < W; ++i) o[i] = P::pack(x[2 * i] / scale, x[(2 * i + 1) % VEC] / scale);
+        if constexpr (VEC == 8) *(u32x2*)p = (u32x2){o[0] | o[1] << 16, o[2] | o[3] << 16};
+        else if constexpr (VEC == 2) *(uint16_t*)p = (uint16_t)o[0];
+        else *(uint8_t*)p = (uint8_t)o[0];
+    }
+};
+
+// Bound by its bytes: every element is read once and written once.  A block takes a few tokens.  A row of a head is cut
+// into pieces: VEC pairs (half layout: two pieces, i and i + half; interleaved: one piece of VEC/2 pairs), or VEC
+// elements behind the rotary part; a thread always works on the same piece of a row, neighbouring threads on
+// neighbouring pieces, then neighbouring heads, so a wavefront moves whole rows.  Rounds go over the (token, head) rows of
+// q, then k, then v: what a round works on is uniform, which keeps its addresses in scalar registers.  The first BATCH
+// rounds are requested before the block makes the cosines and sines of its tokens in LDS (one pair a thread: an angle
+// in float64 costs as much as rotating a dozen heads).
+template <int DT, bool F8, int VEC, bool IL>
+__global__ void __launch_bounds__(APPEND_THREADS) rotary_append_kernel(AppendArgs a) {
+    typedef Piece<DT, VEC> X;
+    __shared__ __align__(16) float cs[APPEND_TOKENS * 128], sn[APPEND_TOKENS * 128];
+    __shared__ int64_t offs[2][APPEND_TOKENS];      // bytes of the token's slot in the pages of k and v, -1: not written
+    __shared__ int32_t skip[APPEND_TOKENS];
+    const int tid = threadIdx.x, half = a.half, hd = a.kv.head_dim;
+    const int64_t t0 = (int64_t)blockIdx.x * a.block_tokens;
+    const int nt = (int)min((int64_t)a.block_tokens, a.tokens - t0);
+    const int np = IL ? 2 * half / VEC : half / VEC, per_head = np + (hd - 2 * half) / VEC;
+    const int slots = APPEND_THREADS / per_head, u = tid % per_head, s0 = tid / per_head;
+    const bool rot = u < np;
+    const int i0 = (rot || IL) ? u * VEC : 2 * half + (u - np) * VEC;       // the piece, and with pairs apart its partner
+    const int i1 = i0 + half;
+    const int rq = (nt * (int)a.role[0].heads + slots - 1) / slots, rk = (nt * (int)a.role[1].heads + slots - 1) / slots;
+    const int r0 = blockIdx.y * a.block_rounds, r1 = min(r0 + a.block_rounds, rq + 2 * rk);
+    X x[BATCH], y[BATCH];
+    int row[BATCH], tok[BATCH];
+    auto request = [&](int first) {
+#pragma unroll
+        for (int n = 0; n < BATCH; ++n) {
+            const int w = first + n, r = w < rq ? 0 : (w < rq + rk ? 1 : 2);
+            const Role& role = a.role[r];
+            const uint32_t i = (uint32_t)(w - (r == 0 ? 0 : (r == 1 ? rq : rq + rk))) * slots + s0;
+            tok[n] = role.magic ? __umulhi(i, role.magic) : i;
+            row[n] = w < r1 && s0 < slots && tok[n] < nt ? (int)(i - tok[n] * role.heads) : -1;
+            if (row[n] >= 0) {
+                const char* p = role.src.ptr + t0 * role.src.token_stride + 2 * i0 +
+                                (uint32_t)(tok[n] * (uint32_t)role.src.token_stride + row[n] * (uint32_t)role.src.head_stride);
+                x[n].load(p);
+                if (!IL && rot) y[n].load(p + 2 * half);
+            }
         }
-        const Heads& dst = is_q ? a.q_out : a.k_out;
-        if (!is_v && dst.ptr && (pos >= 0 || is_q)) {
-            raw* y = (raw*)(dst.ptr + t * dst.token_stride + h * dst.head_stride);
-            y[i0] = pos < 0 ? 0 : E::put(y0);
-            if (pair) y[i1] = pos < 0 ? 0 : E::put(y1);
-        }
-        if (!is_q && page >= 0) {
-            const KvSide& side = is_v ? a.kv.v : a.kv.k;
-            praw* y = (praw*)(side.ptr + page * side.page_stride + h * side.head_stride + slot * side.slot_stride);
-            const float sc = side.scale ? side.scale[h] : 1.f;
-            y[i0] = P::put(y0 / sc);
-            if (pair) y[i1] = P::put(y1 / sc);
+    };
+    request(r0);
+    for (int i = tid; i < nt * half; i += APPEND_THREADS) {
+        const int64_t pos = a.pos[t0 + i / half];
+        const double turn = (double)pos * a.turns[i % half];
+        sincospif(2.f * (float)(turn - rint(turn)), &sn[i], &cs[i]);
+    }
+    if (tid < nt) {
+        const int64_t t = t0 + tid, pos = a.pos[t], s = a.seq ? a.seq[t] : t / a.per_seq;
+        int64_t page = -1;
+        if (s >= 0 && s < a.kv.sequences)
+            page = kv_page_of(a.kv.table + s * a.kv.table_stride, a.kv.reach, a.kv.page_shift, a.kv.num_pages, pos);
+        const int64_t slot = pos & ((1LL << a.kv.page_shift) - 1);
+        offs[0][tid] = page < 0 ? -1 : page * a.kv.k.page_stride + slot * a.kv.k.slot_stride;
+        offs[1][tid] = page < 0 ? -1 : page * a.kv.v.page_stride + slot * a.kv.v.slot_stride;
+        skip[tid] = pos < 0;
+    }
+    __syncthreads();
+    for (int first = r0; first < r1; first += BATCH) {
+        if (first > r0) request(first);
+#pragma unroll
+        for (int n = 0; n < BATCH; ++n) {
+            if (row[n] < 0) continue;
+            const int w = first + n, r = w < rq ? 0 : (w < rq + rk ? 1 : 2);
+            const Role& role = a.role[r];
+            float f0[VEC], f1[VEC];
+            x[n].get(f0);
+            if (!IL && rot) y[n].get(f1);
+            if (rot && r < 2) {
+                const float *c = cs + tok[n] * half + (IL ? i0 / 2 : i0), *s = sn + tok[n] * half + (IL ? i0 / 2 : i0);
+                constexpr int N = IL ? VEC / 2 : VEC;
+                float cc[N], ss[N];
+                if constexpr (N % 4 == 0) {
+#pragma unroll
+                    for (int i = 0; i < N; i += 4) {
+                        const f32x4 cv = *(const f32x4*)(c + i), sv = *(const f32x4*)(s + i);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) cc[i + e] = cv[e], ss[i + e] = sv[e];
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) cc[i] = c[i], ss[i] = s[i];
+                }
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    float& e0 = IL ? f0[2 * i] : f0[i];
+                    float& e1 = IL ? f0[2 * i + 1] : f1[i];
+                    const float p0 = e0, p1 = e1;
+                    e0 = p0 * cc[i] - p1 * ss[i];
+                    e1 = p0 * ss[i] + p1 * cc[i];
+                }
+            }
+            if (r < 2 && role.dst.ptr && (!skip[tok[n]] || (r == 0 && a.zero_skipped))) {
+                char* p = role.dst.ptr + t0 * role.dst.token_stride + 2 * i0 +
+                          (uint32_t)(tok[n] * (uint32_t)role.dst.token_stride + row[n] * (uint32_t)role.dst.head_stride);
+                if (skip[tok[n]]) {
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) f0[i] = f1[i] = 0.f;
+                }
+                X::put(p, f0);
+                if (!IL && rot) X::put(p + 2 * half, f1);
+            }
+            if (r == 0) continue;
+            const int64_t off = offs[r - 1][tok[n]];
+            if (off < 0) continue;
+            const KvSide& side = r == 1 ? a.kv.k : a.kv.v;
+            char* p = side.ptr + off + (int64_t)row[n] * side.head_stride;
+            const float sc = side.scale ? side.scale[row[n]] : 1.f;
+            if constexpr (F8) {
+                X::put_f8(p + i0, f0, sc);
+                if (!IL && rot) X::put_f8(p + i1, f1, sc);
+            } else {
+                if (side.scale) {
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) f0[i] /= sc, f1[i] /= sc;
+                }
+                X::put(p + 2 * i0, f0);
+                if (!IL && rot) X::put(p + 2 * i1, f1);
+            }
         }
     }
 }
 
-// One block per (pair, pool): the page in 16-byte pieces, then its last bytes.
+constexpr int64_t COPY_PIECE = 16384;       // bytes of a block: four 16-byte requests a thread, all before the first store
+
+// One block per (pair, piece of the page, pool).
 __global__ void __launch_bounds__(256) copy_pages_kernel(const char* src_base, int64_t src_pool, int64_t src_page, int64_t src_pages,
                                                          char* dst_base, int64_t dst_pool, int64_t dst_page, int64_t dst_pages,
-                                                         int64_t bytes, const int32_t* src, const int32_t* dst, int wide) {
-    const int64_t s = src[blockIdx.x], d = dst[blockIdx.x];
+                                                         int64_t bytes, int32_t pieces, const int32_t* src, const int32_t* dst,
+                                                         int wide) {
+    const int32_t pair = blockIdx.x / pieces, piece = blockIdx.x % pieces;
+    const int64_t s = src[pair], d = dst[pair];
     if (s < 0 || s >= src_pages || d < 0 || d >= dst_pages) return;
-    const char* from = src_base + (int64_t)blockIdx.y * src_pool + s * src_page;
-    char* to = dst_base + (int64_t)blockIdx.y * dst_pool + d * dst_page;
-    const int64_t n16 = wide ? bytes / 16 : 0;
-    for (int64_t i = threadIdx.x; i < n16; i += 256) ((u32x4*)to)[i] = ((const u32x4*)from)[i];
-    for (int64_t i = 16 * n16 + threadIdx.x; i < bytes; i += 256) to[i] = from[i];
+    const char* from = src_base + (int64_t)blockIdx.y * src_pool + s * src_page + piece * COPY_PIECE;
+    char* to = dst_base + (int64_t)blockIdx.y * dst_pool + d * dst_page + piece * COPY_PIECE;
+    const int64_t n = min(COPY_PIECE, bytes - piece * COPY_PIECE);
+    const int tid = threadIdx.x;
+    if (wide && n == COPY_PIECE) {
+        u32x4 x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = ((const u32x4*)from)[tid + 256 * i];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ((u32x4*)to)[tid + 256 * i] = x[i];
+        return;
+    }
+    const int64_t n16 = wide ? n / 16 : 0;
+    for (int64_t i = tid; i < n16; i += 256) ((u32x4*)to)[i] = ((const u32x4*)from)[i];
+    for (int64_t i = 16 * n16 + tid; i < n; i += 256) to[i] = from[i];
 }
 
-int heads_check(const hyena_heads* h, bool required, const char* name, Heads* out, const char* who) {
-    *out = {nullptr, 0, 0};
-    if (!h || !h->ptr) return required ? hyena_fail(HYENA_EINVAL, "%s: %s is required", who, name) : 0;
-    if (((uintptr_t)h->ptr & 15) || h->token_stride % 8 || h->head_stride % 8)
-        return hyena_fail(HYENA_EALIGN, "%s: %s must be 16-byte aligned with strides of a multiple of 8 elements", who, name);
-    *out = {(char*)h->ptr, h->token_stride * 2, h->head_stride * 2};
-    return 0;
+template <int DT, bool F8, int VEC, bool IL>
+void launch_append(AppendArgs& a, hipStream_t s) {
+    // A block's rounds: up to 2 * BATCH over as many tokens as leave the fewest threads of a round idle, if that makes
+    // enough blocks for every compute unit to hold a few (1024); else fewer, down to one round of one token a block
+    // (the angles of a token are then made in several blocks, which costs less than waiting for one).
+    const int64_t H = a.role[0].heads, K = a.role[1].heads;
+    const int per_head = (IL ? 2 * a.half / VEC : a.half / VEC) + (a.kv.head_dim - 2 * a.half) / VEC;
+    const int64_t slots = APPEND_THREADS / per_head;
+    auto rounds = [&](int64_t nt) { return (nt * H + slots - 1) / slots + 2 * ((nt * K + slots - 1) / slots); };
+    int64_t bt = 1;
+    for (int64_t n = 2; n <= APPEND_TOKENS && rounds(n) <= 2 * BATCH && (a.tokens + n - 1) / n >= 1024; ++n)
+        if (rounds(n) * bt <= rounds(bt) * n) bt = n;
+    int64_t per = rounds(bt);
+    const int64_t blocks = (a.tokens + bt - 1) / bt;
+    const int64_t split = std::min<int64_t>(per, std::max<int64_t>((per + 2 * BATCH - 1) / (2 * BATCH), 1024 / blocks));
+    per = (per + split - 1) / split;
+    a.block_tokens = (int32_t)bt;
+    a.block_rounds = (int32_t)per;
+    hipLaunchKernelGGL((rotary_append_kernel<DT, F8, VEC, IL>), dim3((unsigned)blocks, (unsigned)((rounds(bt) + per - 1) / per)),
+                       dim3(APPEND_THREADS), 0, s, a);
+}
+
+template <int DT, bool F8>
+void launch_append_type(AppendArgs& a, bool il, hipStream_t s) {
+    // pieces of 8 elements where the rotary part allows them, of 2 or 1 where it ends elsewhere
+    const int half = a.half;
+    if (il) {
+        if (half % 4 == 0) launch_append<DT, F8, 8, true>(a, s);
+        else launch_append<DT, F8, 2, true>(a, s);
+    } else {
+        if (half % 8 == 0) launch_append<DT, F8, 8, false>(a, s);
+        else if (half % 2 == 0) launch_append<DT, F8, 2, false>(a, s);
+        else launch_append<DT, F8, 1, false>(a, s);
+    }
 }
 
 }  // namespace
@@ -137,37 +305,44 @@ extern "C" int hyena_rotary_append(const hyena_kv_pages* kv, const hyena_heads* 
     AppendArgs a;
     int rc = kv_pages_check(kv, dtype, &a.kv, who);
     if (rc) return rc;
-    if ((rc = heads_check(q, true, "q", &a.q, who)) || (rc = heads_check(k, true, "k", &a.k, who)) ||
-        (rc = heads_check(v, true, "v", &a.v, who)) || (rc = heads_check(q_out, true, "q_out", &a.q_out, who)) ||
-        (rc = heads_check(k_out, false, "k_out", &a.k_out, who)))
-        return rc;
-    if (!pos || (rotary_dim > 0 && !turns)) return hyena_fail(HYENA_EINVAL, "%s: pos and turns are required", who);
-    if (tokens < 0 || tokens >= (1LL << 31) || heads <= 0 || heads > 65535)
+    if (tokens < 0 || tokens >= (1LL << 31) || heads <= 0)
         return hyena_fail(HYENA_EINVAL, "%s: bad sizes tokens=%lld heads=%lld", who, (long long)tokens, (long long)heads);
+    if (heads > 32768 || kv->kv_heads > 32768) return hyena_fail(HYENA_ENOSUP, "%s: more than 32768 heads", who);
+    if (tokens == 0) return 0;
+    const hyena_heads* in[3] = {q, k, v};
+    const hyena_heads* to[3] = {q_out, k_out, nullptr};
+    const char *in_name[3] = {"q", "k", "v"}, *to_name[3] = {"q_out", "k_out", ""};
+    for (int i = 0; i < 3; ++i) {
+        Role& r = a.role[i];
+        const int64_t n = i == 0 ? heads : kv->kv_heads;
+        if ((rc = kv_heads_check(in[i], true, in_name[i], tokens, n, &r.src, who)) ||
+            (rc = kv_heads_check(to[i], i == 0, to_name[i], tokens, n, &r.dst, who)))
+            return rc;
+        for (const KvHeads* h : {&r.src, &r.dst})       // rows of a block's tokens are addressed with 32 bits
+            if (h->token_stride < 0 || h->head_stride < 0 || APPEND_TOKENS * h->token_stride + n * h->head_stride >= (1LL << 32))
+                return hyena_fail(HYENA_ENOSUP, "%s: rows of %s that lie %lld bytes apart", who, in_name[i],
+                                  (long long)h->token_stride);
+        r.heads = (uint32_t)n;
+        r.magic = n == 1 ? 0 : (uint32_t)(((1ULL << 32) + n - 1) / n);
+    }
+    if (!pos || (rotary_dim > 0 && !turns)) return hyena_fail(HYENA_EINVAL, "%s: pos and turns are required", who);
     if (rotary_dim < 0 || rotary_dim % 2 || rotary_dim > kv->head_dim)
         return hyena_fail(HYENA_EINVAL, "%s: rotary_dim %lld is not an even number up to head_dim %lld", who,
                           (long long)rotary_dim, (long long)kv->head_dim);
-    if (tokens == 0) return 0;
     if (!seq && (kv->sequences == 0 || tokens % kv->sequences))
         return hyena_fail(HYENA_EINVAL, "%s: without seq, tokens (%lld) must be a multiple of the sequences (%lld)", who,
                           (long long)tokens, (long long)kv->sequences);
     a.pos = pos;
     a.seq = seq;
     a.turns = turns;
-    a.heads = (int32_t)heads;
     a.half = (int32_t)(rotary_dim / 2);
     a.per_seq = seq ? 1 : (int32_t)(tokens / kv->sequences);
-    a.interleaved = interleaved != 0;
     a.zero_skipped = zero_skipped != 0;
+    a.tokens = tokens;
     hipStream_t s = (hipStream_t)stream;
-#define RA_CASE(D, P)                                                                                       \
-    if (dtype == D && kv->dtype == P)                                                                       \
-        hipLaunchKernelGGL((rotary_append_kernel<D, P>), dim3((unsigned)tokens), dim3(256), 0, s, a);
-    RA_CASE(HYENA_DTYPE_BF16, HYENA_DTYPE_BF16)
-    RA_CASE(HYENA_DTYPE_F16, HYENA_DTYPE_F16)
-    RA_CASE(HYENA_DTYPE_BF16, HYENA_DTYPE_F8E4M3)
-    RA_CASE(HYENA_DTYPE_F16, HYENA_DTYPE_F8E4M3)
-#undef RA_CASE
+    const bool f8 = kv->dtype == HYENA_DTYPE_F8E4M3, il = interleaved != 0;
+    if (dtype == HYENA_DTYPE_BF16) f8 ? launch_append_type<HYENA_DTYPE_BF16, true>(a, il, s) : launch_append_type<HYENA_DTYPE_BF16, false>(a, il, s);
+    else f8 ? launch_append_type<HYENA_DTYPE_F16, true>(a, il, s) : launch_append_type<HYENA_DTYPE_F16, false>(a, il, s);
     return hyena_check_launch(who);
 }
 
@@ -182,11 +357,16 @@ extern "C" int hyena_kv_copy_pages(const hyena_kv_pools* src_pools, const hyena_
     if (pools == 0 || copies == 0 || page_bytes == 0) return 0;
     if (!src_pools->base || !dst_pools->base || !src || !dst)
         return hyena_fail(HYENA_EINVAL, "%s: pools, src and dst are required", who);
-    const int wide = !(((uintptr_t)src_pools->base | (uintptr_t)dst_pools->base | src_pools->pool_stride | dst_pools->pool_stride |
-                        src_pools->page_stride | dst_pools->page_stride) & 15);
-    hipLaunchKernelGGL(copy_pages_kernel, dim3((unsigned)copies, (unsigned)pools), dim3(256), 0, (hipStream_t)stream,
+    const int64_t at = (int64_t)((uintptr_t)src_pools->base | (uintptr_t)dst_pools->base) |
+                       (pools > 1 ? src_pools->pool_stride | dst_pools->pool_stride : 0) | src_pools->page_stride | dst_pools->page_stride;
+    const int wide = (at & 15) == 0;
+    const int64_t pieces = (page_bytes + COPY_PIECE - 1) / COPY_PIECE;
+    if (copies * pieces >= (1LL << 31))
+        return hyena_fail(HYENA_EINVAL, "%s: %lld copies of %lld bytes are too many for one call", who, (long long)copies,
+                          (long long)page_bytes);
+    hipLaunchKernelGGL(copy_pages_kernel, dim3((unsigned)(copies * pieces), (unsigned)pools), dim3(256), 0, (hipStream_t)stream,
                        (const char*)src_pools->base, src_pools->pool_stride, src_pools->page_stride, src_pools->pages,
                        (char*)dst_pools->base, dst_pools->pool_stride, dst_pools->page_stride, dst_pools->pages, page_bytes,
-                       src, dst, wide);
+                       (int32_t)pieces, src, dst, wide);
     return hyena_check_launch(who);
 }

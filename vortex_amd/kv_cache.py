@@ -9,78 +9,98 @@ hold sequences of any lengths; sequences share pages until one of them writes (f
 Like the functions of ops.py these only enqueue on torch's current stream (of the tensors' device) and keep nothing
 from one call for the next.
 """
-import ctypes
 import math
+import struct
 
 import torch
 
 from . import _lib
-from ._lib import HeadRows, KvPages, KvPools, KvSide
-from .ops import _need_cuda, _strides
 
 _ACT = {torch.bfloat16: _lib.HYENA_DTYPE_BF16, torch.float16: _lib.HYENA_DTYPE_F16}
 _PAGE = {**_ACT, torch.float8_e4m3fn: _lib.HYENA_DTYPE_F8E4M3}
 
-
-class _on:
-    """The stream to enqueue on: the current one of the tensors' device, which is made current for the call."""
-
-    def __init__(self, device):
-        self.guard = torch.cuda.device(device) if device.index != torch.cuda.current_device() else None
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return torch.cuda.current_stream().cuda_stream
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-        return False
+# The argument structures of include/hyena_mi355x.h as packed bytes: built in a quarter of the time ctypes takes for
+# nested Structures, which counts where a call's kernels run for a few microseconds.
+_KV_PAGES = struct.Struct("@P3qP P3qP 4q P3q 2i").pack
+_HEADS = struct.Struct("@P2q").pack
+_POOLS = struct.Struct("@P3q").pack
 
 
-def _same_device(first, *ts):
+# torch.cuda.current_stream builds a Stream object; this returns its handle
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
+def _enqueue(name, index, *args):
+    """Calls an entry point on the current stream of device `index`, which is made current for the call."""
+    fn = getattr(_lib.lib(), name)
+    if index == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        _lib.check(rc, name)
+
+
+def _device(first, *ts):
+    """Index of the one device that all of a call's tensors are on."""
+    index = first.get_device()
+    if index < 0:
+        raise RuntimeError("vortex_amd operators run on the GPU only (got a CPU tensor); there is no CPU fallback")
     for t in ts:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"tensors on {first.device} and {t.device}: all of a call's tensors share one device")
+        if t is not None and t.get_device() != index:
+            raise (RuntimeError if t.get_device() < 0 else ValueError)(
+                f"tensors on {first.device} and {t.device}: all of a call's tensors share one device (GPU only)")
+    return index
 
 
-def _int32(t, name, dim):
-    if t.dtype != torch.int32 or t.dim() != dim or (t.dim() and t.shape[-1] > 1 and t.stride(-1) != 1):
-        raise TypeError(f"{name} must be an int32 tensor of {dim} dimension(s) with contiguous rows, got {tuple(t.shape)} {t.dtype}")
+def _row_stride(t, name, dim):
+    """Checks an int32 vector or matrix with contiguous rows; the matrix's row stride."""
+    if t.dtype is not torch.int32 or t.dim() != dim:
+        raise TypeError(f"{name} must be an int32 tensor of {dim} dimension(s), got {tuple(t.shape)} {t.dtype}")
+    st = t.stride()
+    if st[-1] != 1 and t.shape[-1] > 1:
+        raise ValueError(f"{name} must have contiguous rows")
+    return st[0]
 
 
-def _side(t, scale, heads, name):
-    if t.shape[3] > 1 and t.stride(3) != 1:
-        raise ValueError(f"{name} must be [pages, kv_heads, page_size, head_dim] with contiguous head_dim")
-    if scale is not None and (scale.dtype != torch.float32 or tuple(scale.shape) != (heads,) or not scale.is_contiguous()):
-        raise ValueError(f"the scale of {name} must be a contiguous float32 [{heads}] tensor")
-    p, h, s, _ = _strides(t)
-    return KvSide(t.data_ptr(), p, h, s, None if scale is None else scale.data_ptr())
+def _scale(t, heads, name):
+    if t is None:
+        return 0
+    if t.dtype is not torch.float32 or tuple(t.shape) != (heads,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous float32 [{heads}] tensor")
+    return t.data_ptr()
 
 
 def _kv(k_pages, v_pages, table, k_scale, v_scale, act):
-    """hyena_kv_pages of one layer's cache for activations of type `act`."""
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
+    """hyena_kv_pages of one layer's cache for activations of type `act`, and (kv_heads, head_dim, sequences)."""
+    shape = k_pages.shape
+    if len(shape) != 4 or shape != v_pages.shape:
         raise ValueError("k_pages and v_pages must be [pages, kv_heads, page_size, head_dim] tensors of one shape, got "
                          f"{tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
-    if act not in _ACT or k_pages.dtype != v_pages.dtype or k_pages.dtype not in (act, torch.float8_e4m3fn):
+    dtype = k_pages.dtype
+    if act not in _ACT or v_pages.dtype is not dtype or (dtype is not act and dtype is not torch.float8_e4m3fn):
         raise TypeError("bfloat16 or float16 activations with pages of the same type or of float8_e4m3fn are required, got "
-                        f"{act} with {k_pages.dtype} and {v_pages.dtype}")
-    _int32(table, "table", 2)
-    n, heads, size, hd = k_pages.shape
+                        f"{act} with {dtype} and {v_pages.dtype}")
+    n, heads, size, hd = shape
+    kp, kh, ks, k1 = k_pages.stride()
+    vp, vh, vs, v1 = v_pages.stride()
+    if (k1 != 1 or v1 != 1) and hd > 1:
+        raise ValueError("pages must have contiguous head_dim")
+    row = _row_stride(table, "table", 2)
     rows, width = table.shape
-    return KvPages(_side(k_pages, k_scale, heads, "k_pages"), _side(v_pages, v_scale, heads, "v_pages"), n, size, heads, hd,
-                   table.data_ptr(), table.stride(0) if rows > 1 else width, width, rows, _PAGE[k_pages.dtype], 0)
+    return _KV_PAGES(k_pages.data_ptr(), kp, kh, ks, _scale(k_scale, heads, "k_scale"),
+                     v_pages.data_ptr(), vp, vh, vs, _scale(v_scale, heads, "v_scale"), n, size, heads, hd,
+                     table.data_ptr(), row, width, rows, _PAGE[dtype], 0), heads, hd, rows
 
 
 def _head_rows(t, name, shape, dtype):
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise TypeError(f"{name} is {t.dtype}, expected {dtype}")
-    if tuple(t.shape) != shape or (shape[2] > 1 and t.stride(2) != 1):
+    ts, hs, one = t.stride() if t.dim() == 3 else (0, 0, 0)
+    if t.shape != shape or (one != 1 and shape[2] > 1):
         raise ValueError(f"{name} must be {list(shape)} with contiguous head_dim, got {tuple(t.shape)}")
-    s = _strides(t)
-    return HeadRows(t.data_ptr(), s[0], s[1])
+    return _HEADS(t.data_ptr(), ts, hs)
 
 
 def rotary_turns(rotary_dim, base=10000.0, *, factor=1.0, scaling="linear", original_length=None, slow_turns=1.0,
@@ -127,35 +147,31 @@ def rotary_append(q, k, v, positions, turns, k_pages, v_pages, table, *, seq=Non
     [pages, kv_heads, page_size, hd] of the same type, or float8_e4m3fn holding k / k_scale, v / v_scale (float32
     [kv_heads]).  Returns q_out (rotated q; may be q itself; a new tensor if not given, zero in padding rows);
     k_out, if given, receives the rotated k."""
-    _need_cuda(q, k, v, positions, turns, k_pages, v_pages, table, seq, k_scale, v_scale, q_out, k_out)
-    _same_device(q, k, v, positions, turns, k_pages, v_pages, table, seq, k_scale, v_scale, q_out, k_out)
-    kv = _kv(k_pages, v_pages, table, k_scale, v_scale, q.dtype)
-    if q.dim() != 3 or q.shape[2] != kv.head_dim:
-        raise ValueError(f"q must be [T, heads, {kv.head_dim}], got {tuple(q.shape)}")
-    T, heads, hd = q.shape
-    small = (T, kv.kv_heads, hd)
-    _int32(positions, "positions", 1)
+    index = _device(q, k, v, positions, turns, k_pages, v_pages, table, seq, k_scale, v_scale, q_out, k_out)
+    dtype, shape = q.dtype, q.shape
+    kv, kv_heads, hd, rows = _kv(k_pages, v_pages, table, k_scale, v_scale, dtype)
+    if len(shape) != 3 or shape[2] != hd:
+        raise ValueError(f"q must be [T, heads, {hd}], got {tuple(shape)}")
+    T, heads, _ = shape
+    small = (T, kv_heads, hd)
+    _row_stride(positions, "positions", 1)
     if seq is not None:
-        _int32(seq, "seq", 1)
+        _row_stride(seq, "seq", 1)
     if positions.shape[0] != T or (seq is not None and seq.shape[0] != T):
         raise ValueError(f"{T} rows need {T} positions (and sequences)")
-    if seq is None and (T % kv.sequences if kv.sequences else T):
-        raise ValueError(f"{T} rows over {kv.sequences} sequences: give seq")
-    if turns.dtype != torch.float64 or turns.dim() != 1 or not turns.is_contiguous() or 2 * turns.shape[0] > hd:
+    if seq is None and (T % rows if rows else T):
+        raise ValueError(f"{T} rows over {rows} sequences: give seq")
+    pairs = turns.shape[0] if turns.dim() == 1 else hd
+    if turns.dtype is not torch.float64 or 2 * pairs > hd or not turns.is_contiguous():
         raise ValueError(f"turns must be a contiguous float64 tensor of at most {hd // 2} pairs")
-    qr, kr, vr = _head_rows(q, "q", (T, heads, hd), q.dtype), _head_rows(k, "k", small, q.dtype), _head_rows(v, "v", small, q.dtype)
     zero = q_out is None
     if zero:
-        q_out = torch.empty((T, heads, hd), dtype=q.dtype, device=q.device)
-    qo = _head_rows(q_out, "q_out", (T, heads, hd), q.dtype)
-    ko = None if k_out is None else _head_rows(k_out, "k_out", small, q.dtype)
-    ref = ctypes.byref
-    with _on(q.device) as stream:
-        rc = _lib.lib().hyena_rotary_append(ref(kv), ref(qr), ref(kr), ref(vr), ref(qo), None if ko is None else ref(ko),
-                                            positions.data_ptr(), None if seq is None else seq.data_ptr(), turns.data_ptr(),
-                                            2 * turns.shape[0], int(interleaved), int(zero), T, heads, _ACT[q.dtype], stream)
-    if rc:
-        _lib.check(rc, "hyena_rotary_append")
+        q_out = torch.empty(shape, dtype=dtype, device=q.device)
+    args = (kv, _head_rows(q, "q", shape, dtype), _head_rows(k, "k", small, dtype), _head_rows(v, "v", small, dtype),
+            _head_rows(q_out, "q_out", shape, dtype), None if k_out is None else _head_rows(k_out, "k_out", small, dtype))
+    if T:
+        _enqueue("hyena_rotary_append", index, *args, positions.data_ptr(), None if seq is None else seq.data_ptr(),
+                 turns.data_ptr(), 2 * pairs, bool(interleaved), zero, T, heads, _ACT[dtype])
     return q_out
 
 
@@ -165,41 +181,39 @@ def attn_step(q, k_pages, v_pages, table, lens, *, scale=None, k_scale=None, v_s
     q [B, heads, hd] bf16 or f16; k_pages, v_pages, scales as in rotary_append (append the token's own key first);
     heads a multiple of the pages' kv_heads; table [B, width], lens [B] int32.  scale: of the scores, default
     hd^-1/2.  Returns out [B, heads, hd] of q's type; a sequence with lens <= 0 gets zeros."""
-    _need_cuda(q, k_pages, v_pages, table, lens, k_scale, v_scale, out)
-    _same_device(q, k_pages, v_pages, table, lens, k_scale, v_scale, out)
-    kv = _kv(k_pages, v_pages, table, k_scale, v_scale, q.dtype)
-    if q.dim() != 3 or q.shape[0] != kv.sequences or q.shape[2] != kv.head_dim or q.shape[1] % kv.kv_heads or not q.shape[1]:
-        raise ValueError(f"q must be [{kv.sequences}, a multiple of {kv.kv_heads} heads, {kv.head_dim}], got {tuple(q.shape)}")
-    _int32(lens, "lens", 1)
-    B, heads, hd = q.shape
-    if lens.shape[0] != B:
-        raise ValueError(f"{B} sequences need {B} lengths, got {lens.shape[0]}")
-    qr = _head_rows(q, "q", (B, heads, hd), q.dtype)
+    index = _device(q, k_pages, v_pages, table, lens, k_scale, v_scale, out)
+    dtype, shape = q.dtype, q.shape
+    kv, kv_heads, hd, rows = _kv(k_pages, v_pages, table, k_scale, v_scale, dtype)
+    if len(shape) != 3 or shape[0] != rows or shape[2] != hd or not shape[1] or shape[1] % kv_heads:
+        raise ValueError(f"q must be [{rows}, a multiple of {kv_heads} heads, {hd}], got {tuple(shape)}")
+    _row_stride(lens, "lens", 1)
+    if lens.shape[0] != rows:
+        raise ValueError(f"{rows} sequences need {rows} lengths, got {lens.shape[0]}")
+    heads = shape[1]
+    qr = _head_rows(q, "q", shape, dtype)
     if out is None:
-        out = torch.empty((B, heads, hd), dtype=q.dtype, device=q.device)
-    elif out.dtype != q.dtype or out.shape != q.shape or not out.is_contiguous():
+        out = torch.empty(shape, dtype=dtype, device=q.device)
+    elif out.dtype is not dtype or out.shape != shape or not out.is_contiguous():
         raise ValueError("out must be contiguous and of q's shape and type")
-    L = _lib.lib()
-    nws = L.hyena_attn_step_ws_bytes(B, heads, kv.kv_heads, hd)
-    ws = torch.empty(nws, dtype=torch.uint8, device=q.device) if nws else None
-    with _on(q.device) as stream:
-        rc = L.hyena_attn_step(ctypes.byref(kv), ctypes.byref(qr), lens.data_ptr(), hd ** -0.5 if scale is None else scale,
-                               out.data_ptr(), None if ws is None else ws.data_ptr(), nws, heads, _ACT[q.dtype], stream)
-    if rc:
-        _lib.check(rc, "hyena_attn_step")
+    if rows:
+        nws = _lib.lib().hyena_attn_step_ws_bytes(kv, heads)
+        ws = torch.empty(nws, dtype=torch.uint8, device=q.device) if nws else None
+        _enqueue("hyena_attn_step", index, kv, qr, lens.data_ptr(), hd ** -0.5 if scale is None else scale, out.data_ptr(),
+                 None if ws is None else ws.data_ptr(), nws, heads, _ACT[dtype])
     return out
 
 
 def _pools(t, name):
+    """hyena_kv_pools of [pools, pages, ...], and the bytes of a page."""
     if t.dim() < 3:
         raise ValueError(f"{name} must be [pools, pages, ...], got {tuple(t.shape)}")
-    st, inner = _strides(t), 1
-    for i in range(t.dim() - 1, 1, -1):
-        if st[i] != inner and t.shape[i] != 1:
+    st, shape, inner = t.stride(), t.shape, 1
+    for i in range(len(st) - 1, 1, -1):
+        if st[i] != inner and shape[i] != 1:
             raise ValueError(f"a page of {name} must be contiguous")
-        inner *= t.shape[i]
+        inner *= shape[i]
     es = t.element_size()
-    return KvPools(t.data_ptr(), st[0] * es, st[1] * es, t.shape[1]), inner * es
+    return _POOLS(t.data_ptr(), st[0] * es, st[1] * es, shape[1]), inner * es
 
 
 def kv_copy_pages(pools, src, dst, *, dst_pools=None):
@@ -210,21 +224,18 @@ def kv_copy_pages(pools, src, dst, *, dst_pools=None):
     both a source and a destination).  No page may be a destination twice; pairs with a page that is not there are left
     out.  Returns the pools written to."""
     out = pools if dst_pools is None else dst_pools
-    _need_cuda(pools, src, dst, out)
-    _same_device(pools, src, dst, out)
-    _int32(src, "src", 1)
-    _int32(dst, "dst", 1)
-    if src.shape[0] != dst.shape[0]:
-        raise ValueError(f"{src.shape[0]} source pages, {dst.shape[0]} destination pages")
+    index = _device(pools, src, dst, out)
+    _row_stride(src, "src", 1)
+    _row_stride(dst, "dst", 1)
+    n = src.shape[0]
+    if dst.shape[0] != n:
+        raise ValueError(f"{n} source pages, {dst.shape[0]} destination pages")
     a, size = _pools(pools, "pools")
     b = a
     if dst_pools is not None:
         if out.dtype != pools.dtype or out.dim() != pools.dim() or out.shape[0] != pools.shape[0] or out.shape[2:] != pools.shape[2:]:
             raise ValueError(f"pools {tuple(pools.shape)} {pools.dtype} do not fit dst_pools {tuple(out.shape)} {out.dtype}")
         b, _ = _pools(out, "dst_pools")
-    with _on(pools.device) as stream:
-        rc = _lib.lib().hyena_kv_copy_pages(ctypes.byref(a), ctypes.byref(b), pools.shape[0], size, src.data_ptr(),
-                                            dst.data_ptr(), src.shape[0], stream)
-    if rc:
-        _lib.check(rc, "hyena_kv_copy_pages")
+    if n:
+        _enqueue("hyena_kv_copy_pages", index, a, b, pools.shape[0], size, src.data_ptr(), dst.data_ptr(), n)
     return out
