@@ -457,7 +457,7 @@ int hyena_fir_layer_fwd(const hyena_proj_fwd* proj,
  * A page id outside 0..num_pages-1 names no page: nothing is read from or written to it (attention leaves its positions
  * out, an append drops them), and so do positions beyond table_width*page_size.
  * Rules (others: HYENA_ENOSUP / HYENA_EALIGN): head_dim a multiple of 8 up to 256; page_size a power of two from 16 to
- * 65536; strides multiples of 8 elements (that of a dimension of one element is not looked at), pointers 16-byte
+ * 65536; a table row names at most 2^30 positions; strides multiples of 8 elements (that of a dimension of one element is not looked at), pointers 16-byte
  * aligned. */
 typedef struct hyena_kv_side {
     void* ptr;

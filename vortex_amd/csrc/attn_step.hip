@@ -20,6 +20,7 @@ namespace {
 
 constexpr int WAVES = 4;                    // wavefronts of a block (they share nothing)
 constexpr float LAZY = 8.f;                 // the maximum follows the scores when one exceeds it by more than 2^8
+constexpr int64_t STREAM_BYTES = 128 << 20; // reads beyond this are non-temporal
 
 struct AttnArgs {
     KvPages kv;
@@ -27,8 +28,9 @@ struct AttnArgs {
     int64_t q_seq_stride, q_head_stride;    // bytes
     const int32_t* lens;
     char* out;
-    float* part_o;                          // [2 * wavefronts][rows of a tile][HDP]
-    float* part_ml;                         // [2 * wavefronts][rows of a tile][2]
+    float* part_o;                          // [2 * wavefronts][heads of a tile][HDP]
+    float* part_ml;                         // [2 * wavefronts][heads of a tile][2]
+    int32_t* runs;                          // [sequences][key heads][query tiles][2]: first and last wavefront of a row
     float scale;                            // includes log2(e): the softmax works in powers of two
     int32_t heads, group, qtiles;           // query heads per key head, in tiles of 16
     int32_t waves;
@@ -95,41 +97,45 @@ __device__ __forceinline__ int32_t seq_len(const AttnArgs& a, int32_t b) {
     return (int32_t)min((int64_t)max(a.lens[b], 0), a.kv.reach);
 }
 
-// Sums the tiles of all sequences, 64 lengths at a time, and finds the sequence that holds the first tile of wavefront w,
-// or the one named by `want` where that is not negative.
-__device__ __forceinline__ Place find_place(const AttnArgs& a, int tk_shift, int32_t rows, int64_t w, int32_t want) {
+__device__ __forceinline__ uint32_t scan64(uint32_t x, int lane) {          // inclusive, over the lanes
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t up = __shfl_up(x, o);
+        x += lane >= o ? up : 0;
+    }
+    return x;
+}
+
+// Sums the tiles of all sequences, 64 lengths at a time, and finds the sequence that holds the first tile of wavefront
+// w.  (The tiles of 64 sequences fit 32 bits: kv_pages_check bounds what a table row can name.)
+__device__ __forceinline__ Place find_place(const AttnArgs& a, int tk_shift, int32_t rows, int64_t w) {
     const int lane = lane_id();
     Place p = {0, 0, 0, 0, 0};
     const int32_t B = a.kv.sequences;
+    uint32_t mine = 0, incl = 0;
     for (int32_t b0 = 0; b0 < B; b0 += 64) {
-        int64_t t = 0;
-        if (b0 + lane < B) t = ((int64_t)seq_len(a, b0 + lane) + (1 << tk_shift) - 1) >> tk_shift;
-        for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o);
-        p.total += t;
+        mine = b0 + lane < B ? (uint32_t)(((int64_t)seq_len(a, b0 + lane) + (1 << tk_shift) - 1) >> tk_shift) : 0;
+        incl = scan64(mine, lane);
+        p.total += __builtin_amdgcn_readlane(incl, 63);
     }
-    p.total = uniform(p.total * rows);
+    p.total *= rows;
     p.waves = min(p.total, (int64_t)a.waves);
-    if (want < 0 && w >= p.waves) return p;
-    const int64_t goal = want < 0 ? kv_first_tile(w, p.total, p.waves) : 0;
-    int64_t ahead = 0;
+    if (w >= p.waves) return p;
+    const int64_t goal = kv_first_tile(w, p.total, p.waves);
+    int64_t ahead = 0;                                                      // in tiles per (key head, query tile)
     for (int32_t b0 = 0; b0 < B; b0 += 64) {
-        int32_t mine = 0;
-        if (b0 + lane < B) mine = (int32_t)(((int64_t)seq_len(a, b0 + lane) + (1 << tk_shift) - 1) >> tk_shift);
-        int64_t incl = (int64_t)mine * rows;
-        for (int o = 1; o < 64; o <<= 1) {
-            const int64_t up = __shfl_up(incl, o);
-            if (lane >= o) incl += up;
+        if (B > 64) {
+            mine = b0 + lane < B ? (uint32_t)(((int64_t)seq_len(a, b0 + lane) + (1 << tk_shift) - 1) >> tk_shift) : 0;
+            incl = scan64(mine, lane);
         }
-        const bool here = want < 0 ? ahead + incl > goal : b0 + lane == want;
-        const uint64_t hit = __ballot(here);
+        const uint64_t hit = __ballot((ahead + incl) * rows > goal);
         if (hit) {
             const int l = __builtin_ctzll(hit);
             p.b = b0 + l;
             p.tiles = __builtin_amdgcn_readlane(mine, l);
-            p.first = uniform(ahead + __shfl(incl, l)) - (int64_t)p.tiles * rows;
+            p.first = (ahead + (uint32_t)__builtin_amdgcn_readlane(incl, l) - p.tiles) * rows;
             return p;
         }
-        ahead += uniform(__shfl(incl, 63));
+        ahead += (uint32_t)__builtin_amdgcn_readlane(incl, 63);
     }
     return p;
 }
@@ -146,97 +152,100 @@ struct Walk {
     static constexpr int KW = F8 ? 2 : 4, VW = F8 ? (DL >= 4 ? DL / 4 : 1) : DL / 2;   // dwords of a key / value piece
     static constexpr int ES = F8 ? 1 : 2;
 
+    // What a tile belongs to (wave-uniform).
+    struct Tile {
+        int32_t b, kh, qt, tile, n;         // sequence, key head, query tile, tile of the row, positions of the sequence
+    };
+
     const AttnArgs& a;
     int lane, r, j;                         // lane, lane % 16, lane / 16
-    int32_t n;                              // positions of the sequence
-    const int32_t* table;
-    int32_t ent, ent0;                      // 64 entries of the table row, one a lane, from entry ent0 on
-    const char *kbase, *vbase;              // key head's part of the pages
+    Tile at;                                // the tile that is requested next, or was last
+    int32_t ent_b, ent, ent0;               // 64 entries of the table row of sequence ent_b, one a lane, from entry ent0 on
     uint32_t koff, voff;                    // lane's bytes in a 16-key piece
     uint32_t kmask;                         // PAD: bit c: piece c of this lane is inside the row
-    u32x4 q[NC];
+    u32x4 q[NC], qn[NC];                    // query heads of the row at work, and of the one requested
+    int32_t pg[2 * NT];                     // pages of the requested tile's 16-key pieces
     uint32_t kr[NT][2][NC][KW], vr[NT][8][VB][VW];
     f32x4 o[VB * DL];
-    float m, l, kscale;
-    uint32_t ok;                            // pieces of the tile in the registers whose page is there
-    bool full;                              // every position of that tile counts
+    float m, l;
 
     __device__ __forceinline__ Walk(const AttnArgs& args) : a(args) {
         lane = lane_id();
         r = lane & 15;
         j = lane >> 4;
-    }
-
-    __device__ __forceinline__ void begin(int32_t b, int32_t kh, int32_t qt, int32_t len) {
-        n = len;
-        table = a.kv.table + b * a.kv.table_stride;
-        ent0 = -64;
-        kbase = a.kv.k.ptr + kh * a.kv.k.head_stride;
-        vbase = a.kv.v.ptr + kh * a.kv.v.head_stride;
+        ent_b = -1;
         const int hd = a.kv.head_dim;
         koff = r * (uint32_t)a.kv.k.slot_stride;
         if (!PAD) koff += (K16 ? 16 : 8 * ES) * j;
         const int vd = VB > 1 ? 8 * r : DL * r;
         voff = 4 * j * (uint32_t)a.kv.v.slot_stride + (!PAD || vd < hd ? vd * ES : 0);
-        kscale = a.scale * (a.kv.k.scale ? a.kv.k.scale[kh] : 1.f);
-        const int head = kh * a.group + qt * 16 + r;
-        const bool there = qt * 16 + r < a.group;
-        const char* qp = a.q + b * a.q_seq_stride + (int64_t)(there ? head : kh * a.group) * a.q_head_stride;
         kmask = 0;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            const int d = K16 ? 64 * (c / 2) + 16 * j + 8 * (c % 2) : 32 * c + 8 * j;
-            const bool in = !PAD || d < hd;
-            kmask |= in ? 1u << c : 0;
-            const u32x4 w = *(const u32x4*)(qp + (in ? 2 * d : 0));
-            const u32x4 zero = {0, 0, 0, 0};
-            q[c] = there && in ? w : zero;
-        }
+        for (int c = 0; c < NC; ++c) kmask |= !PAD || key_dim(c) < hd ? 1u << c : 0;
+    }
+    // First element of the 8 that this lane holds of a key row in step c of the product.
+    __device__ __forceinline__ int key_dim(int c) const { return K16 ? 64 * (c / 2) + 16 * j + 8 * (c % 2) : 32 * c + 8 * j; }
+
+    __device__ __forceinline__ void load_q() {
+        const int head = at.qt * 16 + r;
+        const char* p = a.q + at.b * a.q_seq_stride + (int64_t)(at.kh * a.group + (head < a.group ? head : 0)) * a.q_head_stride;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) qn[c] = *(const u32x4*)(p + (!PAD || kmask >> c & 1 ? 2 * key_dim(c) : 0));
+    }
+    __device__ __forceinline__ void start(int32_t qt) {             // of a row: its heads, nothing summed yet
+        const u32x4 zero = {0, 0, 0, 0};
+#pragma unroll
+        for (int c = 0; c < NC; ++c) q[c] = qt * 16 + r < a.group && (!PAD || kmask >> c & 1) ? qn[c] : zero;
 #pragma unroll
         for (int i = 0; i < VB * DL; ++i) o[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
         m = -INFINITY;
         l = 0.f;
     }
 
-    // Base of 16-key piece s (wave-uniform); a piece whose page is not there points at page 0 and is left out later.
+    // Page of a 16-key piece (wave-uniform), or -1.
     __device__ __forceinline__ int32_t page_of(int32_t key0) {
         const int32_t e = key0 >> a.kv.page_shift;
-        if ((uint32_t)(e - ent0) >= 64u) {
+        if (ent_b != at.b || (uint32_t)(e - ent0) >= 64u) {
+            ent_b = at.b;
             ent0 = e;
-            const int64_t at = (int64_t)e + lane, last = ((int64_t)n - 1) >> a.kv.page_shift;
-            ent = at <= last ? table[at] : -1;
+            const int64_t i = (int64_t)e + lane, last = ((int64_t)at.n - 1) >> a.kv.page_shift;
+            ent = i <= last ? a.kv.table[at.b * a.kv.table_stride + i] : -1;
         }
-        return kv_page_or_none(key0 < n ? __builtin_amdgcn_readlane(ent, e - ent0) : -1, a.kv.num_pages);
+        return kv_page_or_none(key0 < at.n ? __builtin_amdgcn_readlane(ent, e - ent0) : -1, a.kv.num_pages);
+    }
+    __device__ __forceinline__ void pages() {
+#pragma unroll
+        for (int s = 0; s < 2 * NT; ++s) pg[s] = page_of(at.tile * TK + 16 * s);
     }
 
-    template <int W> static __device__ __forceinline__ void load(uint32_t (&to)[W], const char* p) {
+    template <bool STREAM, class T> static __device__ __forceinline__ T fetch(const char* p) {
+        if constexpr (STREAM) return __builtin_nontemporal_load((const T*)p);
+        else return *(const T*)p;
+    }
+    template <bool STREAM, int W> static __device__ __forceinline__ void load(uint32_t (&to)[W], const char* p) {
         if constexpr (W == 4) {
-            const u32x4 x = *(const u32x4*)p;
+            const u32x4 x = fetch<STREAM, u32x4>(p);
             to[0] = x[0], to[1] = x[1], to[2] = x[2], to[3] = x[3];
         } else if constexpr (W == 2) {
-            const u32x2 x = *(const u32x2*)p;
+            const u32x2 x = fetch<STREAM, u32x2>(p);
             to[0] = x[0], to[1] = x[1];
         } else if constexpr (F8 && DL == 2) {
-            to[0] = *(const uint16_t*)p;
+            to[0] = fetch<STREAM, uint16_t>(p);
         } else {
-            to[0] = *(const uint32_t*)p;
+            to[0] = fetch<STREAM, uint32_t>(p);
         }
     }
 
-    int32_t pg[2 * NT];
-    __device__ __forceinline__ void pages(int32_t tile) {
-#pragma unroll
-        for (int s = 0; s < 2 * NT; ++s) pg[s] = page_of(tile * TK + 16 * s);
-    }
-    __device__ __forceinline__ void load_keys(int32_t tile) {
+    // A piece whose page is not there is read from page 0 and left out later.
+    template <bool STREAM> __device__ __forceinline__ void load_keys() {
 #pragma unroll
         for (int s = 0; s < 2 * NT; ++s) {
-            const int32_t slot = (tile * TK + 16 * s) & ((1 << a.kv.page_shift) - 1);
-            const char* base = kbase + (int64_t)max(pg[s], 0) * a.kv.k.page_stride + (int64_t)slot * a.kv.k.slot_stride;
+            const int32_t slot = (at.tile * TK + 16 * s) & ((1 << a.kv.page_shift) - 1);
+            const char* base = a.kv.k.ptr + at.kh * a.kv.k.head_stride + (int64_t)max(pg[s], 0) * a.kv.k.page_stride + (int64_t)slot * a.kv.k.slot_stride;
             if constexpr (K16) {
 #pragma unroll
                 for (int c = 0; c < NC / 2; ++c) {
-                    const u32x4 x = *(const u32x4*)(base + (koff + 64 * c));
+                    const u32x4 x = fetch<STREAM, u32x4>(base + (koff + 64 * c));
                     kr[s / 2][s % 2][2 * c][0] = x[0], kr[s / 2][s % 2][2 * c][1] = x[1];
                     kr[s / 2][s % 2][2 * c + 1][0] = x[2], kr[s / 2][s % 2][2 * c + 1][1] = x[3];
                 }
@@ -244,32 +253,25 @@ struct Walk {
 #pragma unroll
                 for (int c = 0; c < NC; ++c) {
                     const uint32_t d = PAD ? (kmask >> c & 1 ? (32 * c + 8 * j) * ES : 0) : 32 * c * ES;
-                    load<KW>(kr[s / 2][s % 2][c], base + (koff + d));
+                    load<STREAM, KW>(kr[s / 2][s % 2][c], base + (koff + d));
                 }
             }
         }
     }
-    __device__ __forceinline__ void load_values(int32_t tile) {
+    template <bool STREAM> __device__ __forceinline__ void load_values() {
 #pragma unroll
         for (int s = 0; s < 2 * NT; ++s) {
-            const int32_t slot = (tile * TK + 16 * s) & ((1 << a.kv.page_shift) - 1);
-            const char* base = vbase + (int64_t)max(pg[s], 0) * a.kv.v.page_stride + (int64_t)slot * a.kv.v.slot_stride;
+            const int32_t slot = (at.tile * TK + 16 * s) & ((1 << a.kv.page_shift) - 1);
+            const char* base = a.kv.v.ptr + at.kh * a.kv.v.head_stride + (int64_t)max(pg[s], 0) * a.kv.v.page_stride + (int64_t)slot * a.kv.v.slot_stride;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int b = 0; b < VB; ++b) {
                     const uint32_t d = PAD && VB > 1 ? (8 * r + 128 * b < a.kv.head_dim ? 128 * b * ES : 0) : 128 * b * ES;
-                    load<VW>(vr[s / 2][4 * (s % 2) + i][b], base + (int64_t)i * a.kv.v.slot_stride + (voff + d));
+                    load<STREAM, VW>(vr[s / 2][4 * (s % 2) + i][b], base + (int64_t)i * a.kv.v.slot_stride + (voff + d));
                 }
         }
     }
-    __device__ __forceinline__ void note(int32_t tile) {
-        ok = 0;
-#pragma unroll
-        for (int s = 0; s < 2 * NT; ++s) ok |= pg[s] >= 0 ? 1u << s : 0;
-        full = ok == (1u << (2 * NT)) - 1 && (tile + 1) * TK <= n;
-    }
-
     // Keys of one piece as the 8 elements of each 32-element step.
     __device__ __forceinline__ u32x4 key_step(const uint32_t (&w)[KW], int c) const {
         u32x4 x;
@@ -286,14 +288,28 @@ struct Walk {
         return x;
     }
 
-    // Tiles [t0, t1) of the row set by begin().
-    __device__ __forceinline__ void run(int32_t t0, int32_t t1) {
-        pages(t0);
-        load_keys(t0);
-        load_values(t0);
-        for (int32_t t = t0; t < t1; ++t) {
-            note(t);
-            const int32_t tn = min(t + 1, t1 - 1);      // the last step loads its own tile once more
+    // `count` tiles from `at` on.  next() moves `at` on by one tile and says whether that is a new row; done(tile, from)
+    // is called after the last tile here of every row, of which the tiles from `from` on are in the sums.  The next
+    // tile is requested while this one is worked on, over the end of a row as well.
+    template <bool STREAM, class Next, class Done>
+    __device__ __forceinline__ void run(int32_t count, Next next, Done done) {
+        pages();
+        load_q();
+        load_keys<STREAM>();
+        load_values<STREAM>();
+        bool fresh = true;
+        int32_t from = 0;
+        while (true) {
+            const Tile t = at;
+            uint32_t ok = 0;                        // pieces of the tile whose page is there
+#pragma unroll
+            for (int s = 0; s < 2 * NT; ++s) ok |= pg[s] >= 0 ? 1u << s : 0;
+            const bool full = ok == (1u << (2 * NT)) - 1 && (t.tile + 1) * TK <= t.n;
+            if (fresh) {
+                start(t.qt);
+                from = t.tile;
+            }
+            const float kscale = a.scale * (a.kv.k.scale ? a.kv.k.scale[t.kh] : 1.f);
             f32x4 s[2 * NT];
 #pragma unroll
             for (int i = 0; i < 2 * NT; ++i) {
@@ -301,8 +317,10 @@ struct Walk {
 #pragma unroll
                 for (int c = 0; c < NC; ++c) s[i] = M::dot(key_step(kr[i / 2][i % 2][c], c), q[c], s[i]);
             }
-            pages(tn);
-            load_keys(tn);
+            if (--count > 0) fresh = next();        // behind the last tile: that one again, unused
+            pages();
+            if (fresh) load_q();
+            load_keys<STREAM>();
             float top = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 2 * NT; ++i)
@@ -313,7 +331,7 @@ struct Walk {
                 for (int i = 0; i < 2 * NT; ++i)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const bool in = (ok >> i & 1) && t * TK + 16 * i + 4 * j + e < n;
+                        const bool in = (ok >> i & 1) && t.tile * TK + 16 * i + 4 * j + e < t.n;
                         s[i][e] = in ? s[i][e] : -INFINITY;
 #pragma unroll
                         for (int b = 0; b < VB; ++b)
@@ -372,21 +390,23 @@ struct Walk {
                         o[b * DL + i] = M::dot(pl, x, o[b * DL + i]);
                     }
             }
-            load_values(tn);
+            load_values<STREAM>();
+            if (count == 0 || fresh) done(t, from);
+            if (count == 0) return;
         }
     }
 
     // The finished row: every head of the tile divided by its sum, rounded and stored.
-    __device__ __forceinline__ void store(int32_t b, int32_t kh, int32_t qt) {
+    __device__ __forceinline__ void store(const Tile& t) {
         typedef KvElem<DT> E;
-        const float sum = sum_over_keys(l), vs = a.kv.v.scale ? a.kv.v.scale[kh] : 1.f;
+        const float sum = sum_over_keys(l), vs = a.kv.v.scale ? a.kv.v.scale[t.kh] : 1.f;
         const float inv = sum != 0.f ? vs / sum : 0.f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int row = 4 * j + e;
             const float f = __shfl(inv, row);
-            if (qt * 16 + row >= a.group) continue;
-            char* y = a.out + ((int64_t)b * a.heads + kh * a.group + qt * 16 + row) * a.kv.head_dim * 2;
+            if (t.qt * 16 + row >= a.group) continue;
+            char* y = a.out + ((int64_t)t.b * a.heads + t.kh * a.group + t.qt * 16 + row) * a.kv.head_dim * 2;
 #pragma unroll
             for (int v = 0; v < VB; ++v) {
                 const int d = VB > 1 ? 8 * r + 128 * v : DL * r;
@@ -425,80 +445,105 @@ struct Walk {
 
 // The tiles of all (sequence, key head, query tile) rows in one line, cut into equal runs, one per wavefront: lengths are
 // on the device, and this is even for any of them.  A row inside one run is finished here; the first and the last row
-// of a run may be parts (slots 2w and 2w + 1).
+// of a run may be parts (slots 2w and 2w + 1), which attn_join_kernel adds up.
 template <int DT, bool F8, int HDP, bool PAD>
 __global__ void __launch_bounds__(64 * WAVES, HDP > 128 ? 1 : 2) attn_walk_kernel(AttnArgs a) {
     typedef Walk<DT, F8, HDP, PAD> W;
     // few tiles are spread over all blocks: the first wavefronts of all blocks come first
     const int64_t w = (int64_t)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * gridDim.x + blockIdx.x;
     const int32_t rows = a.kv.kv_heads * a.qtiles;
-    Place p = find_place(a, W::TK_SHIFT, rows, w, -1);
+    const Place p = find_place(a, W::TK_SHIFT, rows, w);
     if (w >= p.waves) return;
-    int64_t t = kv_first_tile(w, p.total, p.waves);
-    const int64_t end = kv_first_tile(w + 1, p.total, p.waves);
-    int32_t row = (int32_t)((t - p.first) / p.tiles), b = p.b, tiles = p.tiles;
-    int32_t from = (int32_t)(t - p.first - (int64_t)row * tiles);
+    const int64_t t0 = kv_first_tile(w, p.total, p.waves), t1 = kv_first_tile(w + 1, p.total, p.waves);
+    int32_t row = (int32_t)((t0 - p.first) / p.tiles), tiles = p.tiles;
     W walk(a);
-    while (true) {
-        const int32_t kh = row / a.qtiles, qt = row % a.qtiles;
-        const int32_t to = (int32_t)min((int64_t)tiles, from + (end - t));
-        walk.begin(b, kh, qt, seq_len(a, b));
-        walk.run(from, to);
-        if (from == 0 && to == tiles) walk.store(b, kh, qt);
-        else walk.store_part(2 * w + (from == 0), qt);
-        t += to - from;
-        if (t >= end) return;
-        from = 0;
-        if (++row == rows) {
-            row = 0;
-            do {
-                ++b;
-                tiles = (seq_len(a, b) + W::TK - 1) >> W::TK_SHIFT;
-            } while (tiles == 0);       // t < end <= total: a later sequence has tiles
+    walk.at = {p.b, row / a.qtiles, row % a.qtiles, (int32_t)(t0 - p.first - (int64_t)row * tiles), seq_len(a, p.b)};
+    int64_t line = t0 - walk.at.tile;               // of the first tile of the row in `walk.at`
+    int64_t base = line;                            // the same, of the row at work
+    auto next = [&]() {
+        if (++walk.at.tile < tiles) return false;
+        walk.at.tile = 0;
+        line += tiles;
+        if (++walk.at.qt == a.qtiles) {
+            walk.at.qt = 0;
+            if (++walk.at.kh == a.kv.kv_heads) {
+                walk.at.kh = 0;
+                do {                                // another sequence has tiles: the run does not end here
+                    ++walk.at.b;
+                    walk.at.n = seq_len(a, walk.at.b);
+                    tiles = (int32_t)(((int64_t)walk.at.n + W::TK - 1) >> W::TK_SHIFT);
+                } while (tiles == 0);
+            }
         }
-    }
+        return true;
+    };
+    auto done = [&](const typename W::Tile& t, int32_t from) {
+        const int32_t all = (int32_t)(((int64_t)t.n + W::TK - 1) >> W::TK_SHIFT);
+        if (from == 0 && t.tile == all - 1) walk.store(t);
+        else walk.store_part(2 * w + (from == 0), t.qt);
+        if (from == 0 && walk.lane == 0) {
+            int32_t* run = a.runs + (((int64_t)t.b * a.kv.kv_heads + t.kh) * a.qtiles + t.qt) * 2;
+            run[0] = (int32_t)w;
+            run[1] = (int32_t)kv_wave_of_tile(base + all - 1, p.total, p.waves);
+        }
+        base = line;
+    };
+    if (p.total * W::TK * a.kv.head_dim * 2 * W::ES > STREAM_BYTES * a.qtiles) walk.template run<true>((int32_t)(t1 - t0), next, done);
+    else walk.template run<false>((int32_t)(t1 - t0), next, done);
 }
 
-// Rows that lie in several runs: the parts of head `row` weighted by 2^(m - max) and added in the order of the runs.
+// Rows that lie in several runs: the parts of one head weighted by 2^(m - max) and added in the order of the runs.
 // Sequences without a position get zeros here.
 template <int DT, int HDP>
-__global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int tk_shift) {
-    __shared__ float acc[4][HDP], tot[4];
-    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+__global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
+    constexpr int VL = HDP / 4, GROUPS = 256 / VL, AHEAD = 4;       // lanes of a part, parts at a time, and in flight
+    __shared__ __align__(16) float acc[GROUPS][HDP];
+    __shared__ float tot[GROUPS];
+    const int tid = threadIdx.x, lane = tid & 63, grp = tid / VL, d = tid % VL * 4;
     const int32_t b = blockIdx.x / a.heads, head = blockIdx.x % a.heads, kh = head / a.group, in = head % a.group;
-    const int32_t row = kh * a.qtiles + in / 16, hd = a.kv.head_dim, gr = min(a.group, 16);
-    const Place p = find_place(a, tk_shift, a.kv.kv_heads * a.qtiles, 0, b);
+    const int32_t hd = a.kv.head_dim, gr = min(a.group, 16);
     typedef KvElem<DT> E;
     typename E::raw* y = (typename E::raw*)a.out + ((int64_t)b * a.heads + head) * hd;
-    if (p.tiles == 0) {
-        for (int d = tid; d < hd; d += 256) y[d] = 0;
+    const int32_t* run = a.runs + (((int64_t)b * a.kv.kv_heads + kh) * a.qtiles + in / 16) * 2;
+    const int32_t n = seq_len(a, b), w0 = run[0], w1 = run[1];
+    if (n == 0) {
+        if (tid < hd) y[tid] = 0;
         return;
     }
-    const int64_t first = p.first + (int64_t)row * p.tiles;
-    const int64_t w0 = kv_wave_of_tile(first, p.total, p.waves), w1 = kv_wave_of_tile(first + p.tiles - 1, p.total, p.waves);
     if (w0 == w1) return;
+    auto slot = [&](int32_t w) { return (int64_t)(2 * w + (w == w0)) * gr + in % 16; };
     float top = -INFINITY;
-    for (int64_t w = w0 + lane; w <= w1; w += 64) top = fmaxf(top, a.part_ml[((2 * w + (w == w0)) * gr + in % 16) * 2]);
+    for (int32_t w = w0 + lane; w <= w1; w += 64) top = fmaxf(top, a.part_ml[slot(w) * 2]);
     for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
     const float base = top == -INFINITY ? 0.f : top;
-    constexpr int PER = HDP >= 64 ? HDP / 64 : 1;
-    float sum = 0.f, x[PER] = {};
-    for (int64_t w = w0 + wv; w <= w1; w += 4) {
-        const int64_t slot = (2 * w + (w == w0)) * gr + in % 16;
-        const float f = exp2f(a.part_ml[slot * 2] - base);
-        sum += f * a.part_ml[slot * 2 + 1];
+    float sum = 0.f;
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    for (int32_t w = w0 + grp; w <= w1; w += GROUPS * AHEAD) {
+        f32x4 v[AHEAD];
+        float pm[AHEAD], ps[AHEAD];
 #pragma unroll
-        for (int i = 0; i < PER; ++i)
-            if (HDP >= 64 || lane < HDP) x[i] += f * a.part_o[slot * HDP + lane + 64 * i];
+        for (int i = 0; i < AHEAD; ++i) {
+            const int64_t s = slot(min(w + GROUPS * i, w1));
+            v[i] = *(const f32x4*)(a.part_o + s * HDP + d);
+            pm[i] = a.part_ml[s * 2], ps[i] = a.part_ml[s * 2 + 1];
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            if (w + GROUPS * i > w1) continue;
+            const float f = exp2f(pm[i] - base);
+            sum += f * ps[i];
+            x += v[i] * f;
+        }
     }
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-        if (HDP >= 64 || lane < HDP) acc[wv][lane + 64 * i] = x[i];
-    if (lane == 0) tot[wv] = sum;
+    *(f32x4*)&acc[grp][d] = x;
+    if (d == 0) tot[grp] = sum;
     __syncthreads();
-    const float s = (tot[0] + tot[1]) + (tot[2] + tot[3]), vs = a.kv.v.scale ? a.kv.v.scale[kh] : 1.f;
-    const float inv = s != 0.f ? vs / s : 0.f;
-    if (tid < hd) y[tid] = E::put(((acc[0][tid] + acc[1][tid]) + (acc[2][tid] + acc[3][tid])) * inv);
+    if (tid >= hd) return;
+    float s = 0.f, v = 0.f;
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) s += tot[g], v += acc[g][tid];
+    const float vs = a.kv.v.scale ? a.kv.v.scale[kh] : 1.f;
+    y[tid] = E::put(s != 0.f ? v * (vs / s) : 0.f);
 }
 
 int padded(int64_t hd) { return hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
@@ -508,8 +553,7 @@ int waves_for(int64_t hd) { return hd > 128 ? 1024 : 2048; }
 template <int DT, bool F8, int HDP, bool PAD>
 void launch(const AttnArgs& a, hipStream_t s) {
     hipLaunchKernelGGL((attn_walk_kernel<DT, F8, HDP, PAD>), dim3(a.waves / WAVES), dim3(64 * WAVES), 0, s, a);
-    hipLaunchKernelGGL((attn_join_kernel<DT, HDP>), dim3((unsigned)a.kv.sequences * a.heads), dim3(256), 0, s, a,
-                       Walk<DT, F8, HDP, PAD>::TK_SHIFT);
+    hipLaunchKernelGGL((attn_join_kernel<DT, HDP>), dim3((unsigned)a.kv.sequences * a.heads), dim3(256), 0, s, a);
 }
 
 template <int DT, bool F8>
@@ -528,7 +572,8 @@ extern "C" int64_t hyena_attn_step_ws_bytes(const hyena_kv_pages* kv, int64_t he
     if (!kv || kv->sequences <= 0 || heads <= 0 || kv->kv_heads <= 0 || kv->head_dim <= 0 || kv->head_dim > 256 || heads % kv->kv_heads)
         return 0;
     const int64_t g = heads / kv->kv_heads, rows = g < 16 ? g : 16;
-    return 2 * (int64_t)waves_for(kv->head_dim) * rows * (padded(kv->head_dim) + 2) * 4;
+    return 2 * (int64_t)waves_for(kv->head_dim) * rows * (padded(kv->head_dim) + 2) * 4 +
+           kv->sequences * kv->kv_heads * ((g + 15) / 16) * 8;
 }
 
 extern "C" int hyena_attn_step(const hyena_kv_pages* kv, const hyena_heads* q, const int32_t* lens, float scale, void* out,
@@ -562,6 +607,7 @@ extern "C" int hyena_attn_step(const hyena_kv_pages* kv, const hyena_heads* q, c
     a.waves = waves_for(kv->head_dim);
     a.part_o = (float*)ws;
     a.part_ml = a.part_o + 2 * (int64_t)a.waves * (a.group < 16 ? a.group : 16) * padded(kv->head_dim);
+    a.runs = (int32_t*)(a.part_ml + 4 * (int64_t)a.waves * (a.group < 16 ? a.group : 16));
     const bool f8 = kv->dtype == HYENA_DTYPE_F8E4M3;
     // the plain form loads 16 bytes of a row at a time and whole rows; other row lengths and, in 8 bits, strides that
     // are only 8-byte multiples take the form that masks the pieces behind a row's end

@@ -20,6 +20,8 @@ int kv_pages_check(const hyena_kv_pages* kv, int dtype, KvPages* out, const char
         return hyena_fail(HYENA_ENOSUP, "%s: head_dim %lld is not a multiple of 8 up to 256", who, (long long)kv->head_dim);
     if (kv->page_size < 16 || kv->page_size > 65536 || (kv->page_size & (kv->page_size - 1)) != 0)
         return hyena_fail(HYENA_ENOSUP, "%s: page_size %lld is not a power of two from 16 to 65536", who, (long long)kv->page_size);
+    if (kv->table_width > (1LL << 30) / kv->page_size)
+        return hyena_fail(HYENA_ENOSUP, "%s: a table row of %lld pages names more than 2^30 positions", who, (long long)kv->table_width);
     const int64_t es = kv_elem_bytes(kv->dtype);
     const hyena_kv_side* in[2] = {&kv->k, &kv->v};
     KvSide* to[2] = {&out->k, &out->v};
@@ -125,6 +127,11 @@ __global__ void __launch_bounds__(APPEND_THREADS) rotary_append_kernel(AppendArg
     const int tid = threadIdx.x, half = a.half, hd = a.kv.head_dim;
     const int64_t t0 = (int64_t)blockIdx.x * a.block_tokens;
     const int nt = (int)min((int64_t)a.block_tokens, a.tokens - t0);
+    if (!a.zero_skipped) {                          // a block of padding rows reads none of them
+        bool any = false;
+        for (int i = 0; i < nt; ++i) any |= a.pos[t0 + i] >= 0;
+        if (!any) return;
+    }
     const int np = IL ? 2 * half / VEC : half / VEC, per_head = np + (hd - 2 * half) / VEC;
     const int slots = APPEND_THREADS / per_head, u = tid % per_head, s0 = tid / per_head;
     const bool rot = u < np;
