@@ -69,6 +69,8 @@ const char* hyena_last_error_string(void);
  *   "cl_f32_mfma"                               float32 tensors in hyena_fir_cl_fwd_dtype: 0 = always the direct form,
  *                                               1 / 2 = the matrix-core form with one tile per block / blocks that walk
  *                                               a ring of tiles, wherever the matrix-core form applies
+ *   "attn_short"                                hyena_attn_step: 0 = the even cut over all wavefronts with its join, 1 = one
+ *                                               block per (sequence, key head), for any length
  * Returns 0, or HYENA_EINVAL for an unknown name. */
 int hyena_set_launch_override(const char* name, int64_t value);
 

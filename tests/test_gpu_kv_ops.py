@@ -78,6 +78,21 @@ def test_attention_long_and_ragged_batches(lens):
     assert torch.equal(a, b)                    # the order of every sum is fixed
 
 
+@pytest.mark.parametrize("form", [0, 1])
+@pytest.mark.parametrize("dtype,fp8", [(BF, False), (F16, True)])
+@pytest.mark.parametrize("kv_heads,group,hd,page", [(2, 1, 128, 16), (1, 8, 64, 64), (1, 17, 32, 16), (2, 3, 256, 32), (1, 5, 80, 16),
+                                                    (1, 2, 136, 16)])
+def test_attention_both_launch_forms(override, kv_heads, group, hd, page, dtype, fp8, form):
+    override(attn_short=form)
+    lens = [0, 1, 33, 700, 2500, 64, 256, 257]
+    c = cache(hd + group, lens, kv_heads, hd, page, dtype, fp8)
+    q = (2 * torch.randn(len(lens), kv_heads * group, hd, generator=gen(17))).to(dtype).to(DEV)
+    check_attn(q, c, lens)
+    c[2][3, 5], c[2][4, :] = -1, -1             # a page that is not there, a sequence without any
+    got = check_attn(q, c, lens)
+    assert float(got[4].abs().max()) == 0.0
+
+
 def test_attention_sharp_and_flat_scores():
     lens = [700, 333]
     c = cache(5, lens, 2, 64, 32, BF)

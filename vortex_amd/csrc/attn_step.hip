@@ -3,7 +3,7 @@
 //   s_j = scale * <q, K_j>,  o = sum_j 2^(s_j - m) V_j / sum_j 2^(s_j - m)     (scale includes log2 e)
 //
 // Bound by the bytes of K and V: one multiply-add per stored element and query head.  Everything is laid out so that
-// each wavefront streams pages through registers with no LDS and no barrier:
+// each wavefront streams pages through its registers without a barrier:
 //   * S^T = K Q^T on v_mfma_f32_16x16x32: a lane holds 8 consecutive elements of ONE key (16 bytes as they lie in the
 //     page), the columns are up to 16 query heads that share the key head;
 //   * the result leaves key 4*(lane/16) + i of a 16-key piece in register i of lane `lane`, column lane % 16 -- which is
@@ -33,7 +33,7 @@ struct AttnArgs {
     int32_t* runs;                          // [sequences][key heads][query tiles][2]: first and last wavefront of a row
     float scale;                            // includes log2(e): the softmax works in powers of two
     int32_t heads, group, qtiles;           // query heads per key head, in tiles of 16
-    int32_t waves;
+    int32_t waves;                          // of the even cut
 };
 
 template <int DT> struct Mma;
@@ -148,9 +148,17 @@ struct Walk {
     static constexpr int VB = HDP > 128 ? HDP / 128 : 1;            // such blocks in a row
     static constexpr int NT = F8 ? (HDP >= 256 ? 1 : HDP == 128 ? 2 : 4) : (HDP >= 128 ? 1 : HDP == 64 ? 2 : 4);
     static constexpr int TK = 32 * NT, TK_SHIFT = NT == 1 ? 5 : NT == 2 ? 6 : 7;
-    static constexpr bool K16 = F8 && !PAD && HDP >= 64;            // e4m3 keys in 16-byte loads
+    static constexpr bool K16 = F8 && !PAD && HDP >= 64;            // e4m3 keys in 16-byte pieces
     static constexpr int KW = F8 ? 2 : 4, VW = F8 ? (DL >= 4 ? DL / 4 : 1) : DL / 2;   // dwords of a key / value piece
     static constexpr int ES = F8 ? 1 : 2;
+    // The products want consecutive lanes on different keys (and 8-bit values 8 bytes a lane): requests like that are
+    // slow in the address unit (e4m3: 5.0 against 5.9 TB/s).  So rows are requested in 64 consecutive 16-byte pieces and
+    // turned around in an LDS buffer of the wavefront, 16 rows at a time, two buffers in turn.  Piece x of row y lies at
+    // x ^ row_swizzle(y), which spreads the reads over the banks.  (LDS operations of a wavefront stay in order.)
+    static constexpr int RB = HDP * ES, CPR = RB / 16;              // bytes and 16-byte pieces of a row
+    static constexpr bool TURN = !PAD && CPR >= 4, TURNV = TURN && F8;
+    static constexpr int LDS_BYTES = TURN ? 2 * 16 * RB : 0;        // of a wavefront
+    static __device__ __forceinline__ int row_swizzle(int row) { return (RB >= 256 ? row : row / (256 / RB)) & (CPR - 1) & 15; }
 
     // What a tile belongs to (wave-uniform).
     struct Tile {
@@ -161,24 +169,34 @@ struct Walk {
     int lane, r, j;                         // lane, lane % 16, lane / 16
     Tile at;                                // the tile that is requested next, or was last
     int32_t ent_b, ent, ent0;               // 64 entries of the table row of sequence ent_b, one a lane, from entry ent0 on
-    uint32_t koff, voff;                    // lane's bytes in a 16-key piece
+    uint32_t koff[TURN ? CPR / 4 : 1], voff[TURNV ? CPR / 4 : 1];   // lane's bytes in a 16-key piece
+    char* lds;                              // this wavefront's part of the LDS
     uint32_t kmask;                         // PAD: bit c: piece c of this lane is inside the row
     u32x4 q[NC], qn[NC];                    // query heads of the row at work, and of the one requested
     int32_t pg[2 * NT];                     // pages of the requested tile's 16-key pieces
-    uint32_t kr[NT][2][NC][KW], vr[NT][8][VB][VW];
+    uint32_t kr[TURN ? 1 : NT][2][NC][KW], vr[NT][8][VB][VW];
+    u32x4 kt[TURN ? 2 * NT : 1][TURN ? CPR / 4 : 1], vt[TURNV ? 2 * NT : 1][TURNV ? CPR / 4 : 1];
     f32x4 o[VB * DL];
     float m, l;
 
-    __device__ __forceinline__ Walk(const AttnArgs& args) : a(args) {
+    __device__ __forceinline__ Walk(const AttnArgs& args, char* buf) : a(args), lds(buf) {
         lane = lane_id();
         r = lane & 15;
         j = lane >> 4;
         ent_b = -1;
         const int hd = a.kv.head_dim;
-        koff = r * (uint32_t)a.kv.k.slot_stride;
-        if (!PAD) koff += (K16 ? 16 : 8 * ES) * j;
+        if constexpr (TURN) {
+#pragma unroll
+            for (int i = 0; i < CPR / 4; ++i) {
+                const int row = (64 * i + lane) / CPR, x = 16 * (lane % CPR ^ row_swizzle(row));
+                koff[i] = row * (uint32_t)a.kv.k.slot_stride + x;
+                if constexpr (TURNV) voff[i] = row * (uint32_t)a.kv.v.slot_stride + x;
+            }
+        } else {
+            koff[0] = r * (uint32_t)a.kv.k.slot_stride + (PAD ? 0 : 8 * ES * j);
+        }
         const int vd = VB > 1 ? 8 * r : DL * r;
-        voff = 4 * j * (uint32_t)a.kv.v.slot_stride + (!PAD || vd < hd ? vd * ES : 0);
+        if (!TURNV) voff[0] = 4 * j * (uint32_t)a.kv.v.slot_stride + (!PAD || vd < hd ? vd * ES : 0);
         kmask = 0;
 #pragma unroll
         for (int c = 0; c < NC; ++c) kmask |= !PAD || key_dim(c) < hd ? 1u << c : 0;
@@ -196,6 +214,9 @@ struct Walk {
         const u32x4 zero = {0, 0, 0, 0};
 #pragma unroll
         for (int c = 0; c < NC; ++c) q[c] = qt * 16 + r < a.group && (!PAD || kmask >> c & 1) ? qn[c] : zero;
+        nothing();
+    }
+    __device__ __forceinline__ void nothing() {
 #pragma unroll
         for (int i = 0; i < VB * DL; ++i) o[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
         m = -INFINITY;
@@ -210,6 +231,7 @@ struct Walk {
             ent0 = e;
             const int64_t i = (int64_t)e + lane, last = ((int64_t)at.n - 1) >> a.kv.page_shift;
             ent = i <= last ? a.kv.table[at.b * a.kv.table_stride + i] : -1;
+            asm volatile("" : "+v"(ent));       // wait for it here: a wait at its use would hold up every tile
         }
         return kv_page_or_none(key0 < at.n ? __builtin_amdgcn_readlane(ent, e - ent0) : -1, a.kv.num_pages);
     }
@@ -242,18 +264,14 @@ struct Walk {
         for (int s = 0; s < 2 * NT; ++s) {
             const int32_t slot = (at.tile * TK + 16 * s) & ((1 << a.kv.page_shift) - 1);
             const char* base = a.kv.k.ptr + at.kh * a.kv.k.head_stride + (int64_t)max(pg[s], 0) * a.kv.k.page_stride + (int64_t)slot * a.kv.k.slot_stride;
-            if constexpr (K16) {
+            if constexpr (TURN) {
 #pragma unroll
-                for (int c = 0; c < NC / 2; ++c) {
-                    const u32x4 x = fetch<STREAM, u32x4>(base + (koff + 64 * c));
-                    kr[s / 2][s % 2][2 * c][0] = x[0], kr[s / 2][s % 2][2 * c][1] = x[1];
-                    kr[s / 2][s % 2][2 * c + 1][0] = x[2], kr[s / 2][s % 2][2 * c + 1][1] = x[3];
-                }
+                for (int i = 0; i < CPR / 4; ++i) kt[s][i] = fetch<STREAM, u32x4>(base + koff[i]);
             } else {
 #pragma unroll
                 for (int c = 0; c < NC; ++c) {
                     const uint32_t d = PAD ? (kmask >> c & 1 ? (32 * c + 8 * j) * ES : 0) : 32 * c * ES;
-                    load<STREAM, KW>(kr[s / 2][s % 2][c], base + (koff + d));
+                    load<STREAM, KW>(kr[s / 2][s % 2][c], base + (koff[0] + d));
                 }
             }
         }
@@ -263,18 +281,59 @@ struct Walk {
         for (int s = 0; s < 2 * NT; ++s) {
             const int32_t slot = (at.tile * TK + 16 * s) & ((1 << a.kv.page_shift) - 1);
             const char* base = a.kv.v.ptr + at.kh * a.kv.v.head_stride + (int64_t)max(pg[s], 0) * a.kv.v.page_stride + (int64_t)slot * a.kv.v.slot_stride;
+            if constexpr (TURNV) {
+#pragma unroll
+                for (int i = 0; i < CPR / 4; ++i) vt[s][i] = fetch<STREAM, u32x4>(base + voff[i]);
+                continue;
+            }
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int b = 0; b < VB; ++b) {
                     const uint32_t d = PAD && VB > 1 ? (8 * r + 128 * b < a.kv.head_dim ? 128 * b * ES : 0) : 128 * b * ES;
-                    load<STREAM, VW>(vr[s / 2][4 * (s % 2) + i][b], base + (int64_t)i * a.kv.v.slot_stride + (voff + d));
+                    load<STREAM, VW>(vr[s / 2][4 * (s % 2) + i][b], base + (int64_t)i * a.kv.v.slot_stride + (voff[0] + d));
                 }
         }
     }
-    // Keys of one piece as the 8 elements of each 32-element step.
-    __device__ __forceinline__ u32x4 key_step(const uint32_t (&w)[KW], int c) const {
+    // 16 rows into the buffer of piece s.
+    __device__ __forceinline__ void turn(int s, const u32x4 (&rows)[CPR / 4 ? CPR / 4 : 1]) {
+#pragma unroll
+        for (int i = 0; i < CPR / 4; ++i) *(u32x4*)(lds + s % 2 * 16 * RB + i * 1024 + lane * 16) = rows[i];
+    }
+    // The values of a tile, 8 bytes a lane: elements 8 * (lane % 16) .. of rows 4 * (lane / 16) + 0..3 of every piece.
+    __device__ __forceinline__ void turn_values() {
+        if constexpr (TURNV) {
+#pragma unroll
+            for (int s = 0; s < 2 * NT; ++s) {
+                turn(s, vt[s]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int b = 0; b < VB; ++b) {
+                        const int row = 4 * j + i, byte = VB > 1 ? 8 * r + 128 * b : DL * r;
+                        const char* p = lds + s % 2 * 16 * RB + row * RB + 16 * (byte / 16 ^ row_swizzle(row)) + byte % 16;
+                        if constexpr (VW == 2) {
+                            const u32x2 x = *(const u32x2*)p;
+                            vr[s / 2][4 * (s % 2) + i][b][0] = x[0], vr[s / 2][4 * (s % 2) + i][b][1] = x[1];
+                        } else {
+                            vr[s / 2][4 * (s % 2) + i][b][0] = *(const uint32_t*)p;
+                        }
+                    }
+            }
+        }
+    }
+    // The 8 elements of step c of a lane's key in 16-key piece s.
+    __device__ __forceinline__ u32x4 key_step(int s, int c) const {
         u32x4 x;
+        uint32_t w[KW];
+        if constexpr (TURN) {
+            const u32x4 y = *(const u32x4*)(lds + s % 2 * 16 * RB + r * RB + 16 * ((4 * (K16 ? c / 2 : c) + j) ^ row_swizzle(r)));
+#pragma unroll
+            for (int i = 0; i < KW; ++i) w[i] = y[K16 ? 2 * (c % 2) + i : i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < KW; ++i) w[i] = kr[s / 2][s % 2][c][i];
+        }
         if constexpr (F8) {
             x[0] = M::template from_f8<false>(w[0]), x[1] = M::template from_f8<true>(w[0]);
             x[2] = M::template from_f8<false>(w[1]), x[3] = M::template from_f8<true>(w[1]);
@@ -299,6 +358,7 @@ struct Walk {
         load_values<STREAM>();
         bool fresh = true;
         int32_t from = 0;
+        float kscale = 0.f;
         while (true) {
             const Tile t = at;
             uint32_t ok = 0;                        // pieces of the tile whose page is there
@@ -308,19 +368,21 @@ struct Walk {
             if (fresh) {
                 start(t.qt);
                 from = t.tile;
+                kscale = a.scale * (a.kv.k.scale ? a.kv.k.scale[t.kh] : 1.f);
             }
-            const float kscale = a.scale * (a.kv.k.scale ? a.kv.k.scale[t.kh] : 1.f);
             f32x4 s[2 * NT];
 #pragma unroll
             for (int i = 0; i < 2 * NT; ++i) {
                 s[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+                if constexpr (TURN) turn(i, kt[i]);
 #pragma unroll
-                for (int c = 0; c < NC; ++c) s[i] = M::dot(key_step(kr[i / 2][i % 2][c], c), q[c], s[i]);
+                for (int c = 0; c < NC; ++c) s[i] = M::dot(key_step(i, c), q[c], s[i]);
             }
             if (--count > 0) fresh = next();        // behind the last tile: that one again, unused
             pages();
             if (fresh) load_q();
             load_keys<STREAM>();
+            turn_values();
             float top = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 2 * NT; ++i)
@@ -344,7 +406,7 @@ struct Walk {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) top = fmaxf(top, s[i][e]);
             if (__any(top > m + LAZY)) {                // the maximum moves for all heads of the tile at once
-                const float mn = fmaxf(m, max_over_keys(top)), f = exp2f(m - (mn == -INFINITY ? 0.f : mn));
+                const float mn = fmaxf(m, max_over_keys(top)), f = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
                 m = mn;
                 l *= f;
                 const f32x4 g = {__shfl(f, 4 * j), __shfl(f, 4 * j + 1), __shfl(f, 4 * j + 2), __shfl(f, 4 * j + 3)};
@@ -356,7 +418,7 @@ struct Walk {
             for (int i = 0; i < 2 * NT; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    s[i][e] = exp2f(s[i][e] - base);
+                    s[i][e] = __builtin_amdgcn_exp2f(s[i][e] - base);
                     l += s[i][e];
                 }
 #pragma unroll
@@ -456,7 +518,8 @@ __global__ void __launch_bounds__(64 * WAVES, HDP > 128 ? 1 : 2) attn_walk_kerne
     if (w >= p.waves) return;
     const int64_t t0 = kv_first_tile(w, p.total, p.waves), t1 = kv_first_tile(w + 1, p.total, p.waves);
     int32_t row = (int32_t)((t0 - p.first) / p.tiles), tiles = p.tiles;
-    W walk(a);
+    __shared__ __align__(16) char lds[W::LDS_BYTES ? WAVES * W::LDS_BYTES : 16];
+    W walk(a, lds + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * W::LDS_BYTES);
     walk.at = {p.b, row / a.qtiles, row % a.qtiles, (int32_t)(t0 - p.first - (int64_t)row * tiles), seq_len(a, p.b)};
     int64_t line = t0 - walk.at.tile;               // of the first tile of the row in `walk.at`
     int64_t base = line;                            // the same, of the row at work
@@ -484,12 +547,70 @@ __global__ void __launch_bounds__(64 * WAVES, HDP > 128 ? 1 : 2) attn_walk_kerne
         if (from == 0 && walk.lane == 0) {
             int32_t* run = a.runs + (((int64_t)t.b * a.kv.kv_heads + t.kh) * a.qtiles + t.qt) * 2;
             run[0] = (int32_t)w;
-            run[1] = (int32_t)kv_wave_of_tile(base + all - 1, p.total, p.waves);
+            run[1] = (int32_t)(t.tile == all - 1 ? w : kv_wave_of_tile(base + all - 1, p.total, p.waves));
         }
         base = line;
     };
     if (p.total * W::TK * a.kv.head_dim * 2 * W::ES > STREAM_BYTES * a.qtiles) walk.template run<true>((int32_t)(t1 - t0), next, done);
     else walk.template run<false>((int32_t)(t1 - t0), next, done);
+}
+
+// Short rows: one block per row, its wavefronts take the tiles in turn and add up their parts in LDS.  One launch.
+template <int HDP> constexpr int short_waves() { return HDP > 128 ? 4 : 8; }
+
+template <int DT, bool F8, int HDP, bool PAD>
+__global__ void __launch_bounds__(64 * short_waves<HDP>()) attn_short_kernel(AttnArgs a) {
+    typedef Walk<DT, F8, HDP, PAD> W;
+    constexpr int N = short_waves<HDP>(), BYTES = W::LDS_BYTES > 16 * HDP * 4 ? W::LDS_BYTES : 16 * HDP * 4;
+    __shared__ __align__(16) char lds[N * BYTES];               // to turn rows around, then [wavefront][head][HDP] sums
+    __shared__ float ms[N][16], ls[N][16];
+    const int tid = threadIdx.x, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int32_t qt = blockIdx.x % a.qtiles, kh = blockIdx.x / a.qtiles % a.kv.kv_heads, b = blockIdx.x / a.qtiles / a.kv.kv_heads;
+    const int32_t n = seq_len(a, b), tiles = (int32_t)(((int64_t)n + W::TK - 1) >> W::TK_SHIFT), hd = a.kv.head_dim;
+    W walk(a, lds + wv * BYTES);
+    walk.at = {b, kh, qt, wv, n};
+    if (wv < tiles) {
+        auto next = [&]() { walk.at.tile += N; return false; };
+        auto done = [](const typename W::Tile&, int32_t) {};
+        walk.template run<false>((tiles - wv + N - 1) / N, next, done);
+    } else {
+        walk.nothing();
+    }
+    const float sum = sum_over_keys(walk.l);
+    if (walk.j == 0) ms[wv][walk.r] = walk.m, ls[wv][walk.r] = sum;
+    __syncthreads();
+    const int rows = min(a.group - qt * 16, 16);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int row = 4 * walk.j + e;
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < N; ++w) top = fmaxf(top, ms[w][row]);
+        const float f = __builtin_amdgcn_exp2f(ms[wv][row] - (top == -INFINITY ? 0.f : top));
+        if (row >= rows) continue;
+        float* y = (float*)lds + (wv * 16 + row) * HDP;
+#pragma unroll
+        for (int v = 0; v < W::VB; ++v)
+#pragma unroll
+            for (int i = 0; i < W::DL; ++i) y[(W::VB > 1 ? 8 * walk.r + 128 * v : W::DL * walk.r) + i] = walk.o[v * W::DL + i][e] * f;
+    }
+    __syncthreads();
+    const float vs = a.kv.v.scale ? a.kv.v.scale[kh] : 1.f;
+    for (int x = tid; x < rows * HDP; x += 64 * N) {
+        const int row = x / HDP, d = x % HDP;
+        if (d >= hd) continue;
+        float top = -INFINITY, s = 0.f, v = 0.f;
+#pragma unroll
+        for (int w = 0; w < N; ++w) top = fmaxf(top, ms[w][row]);
+        top = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int w = 0; w < N; ++w) {
+            s += ls[w][row] * __builtin_amdgcn_exp2f(ms[w][row] - top);
+            v += ((const float*)lds)[(w * 16 + row) * HDP + d];
+        }
+        typedef KvElem<DT> E;
+        ((typename E::raw*)a.out)[((int64_t)b * a.heads + kh * a.group + qt * 16 + row) * hd + d] = E::put(s != 0.f ? v * (vs / s) : 0.f);
+    }
 }
 
 // Rows that lie in several runs: the parts of one head weighted by 2^(m - max) and added in the order of the runs.
@@ -530,7 +651,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
             if (w + GROUPS * i > w1) continue;
-            const float f = exp2f(pm[i] - base);
+            const float f = __builtin_amdgcn_exp2f(pm[i] - base);
             sum += f * ps[i];
             x += v[i] * f;
         }
@@ -548,21 +669,42 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
 
 int padded(int64_t hd) { return hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
 
-int waves_for(int64_t hd) { return hd > 128 ? 1024 : 2048; }
+// Whether every row is short: what the table can name (lengths are on the device) keeps a block's wavefronts at a few
+// tiles each, and the blocks are few enough to run at once or nearly.
+bool short_rows(const hyena_kv_pages* kv, int64_t heads) {
+    const int64_t ov = hyena_override(HYENA_OV_ATTN_SHORT);
+    if (ov >= 0) return ov != 0;
+    const int64_t rows = kv->sequences * kv->kv_heads * ((heads / kv->kv_heads + 15) / 16);
+    const int64_t bytes = kv->table_width * kv->page_size * kv->head_dim * 2 * kv_elem_bytes(kv->dtype);   // of a row
+    return bytes <= (512 << 10) && rows <= 512;
+}
+
+// Wavefronts of the even cut.  One per SIMD reads long rows fastest (1.07 GB in 256 rows: e4m3 196 us against 202 with
+// two, bf16 174 against 180) and leaves fewer parts to join; with many rows each wavefront changes rows often, and a
+// second one on the SIMD works meanwhile (2048 rows of up to 4096 keys: 372 us against 397 with one).
+int64_t waves_for(const hyena_kv_pages* kv, int64_t heads) {
+    const int64_t rows = kv->sequences * kv->kv_heads * ((heads / kv->kv_heads + 15) / 16);
+    return kv->head_dim <= 128 && rows > 1024 ? 2048 : 1024;
+}
 
 template <int DT, bool F8, int HDP, bool PAD>
-void launch(const AttnArgs& a, hipStream_t s) {
+void launch(const AttnArgs& a, bool few, hipStream_t s) {
+    if (few) {
+        hipLaunchKernelGGL((attn_short_kernel<DT, F8, HDP, PAD>), dim3((unsigned)a.kv.sequences * a.kv.kv_heads * a.qtiles),
+                           dim3(64 * short_waves<HDP>()), 0, s, a);
+        return;
+    }
     hipLaunchKernelGGL((attn_walk_kernel<DT, F8, HDP, PAD>), dim3(a.waves / WAVES), dim3(64 * WAVES), 0, s, a);
     hipLaunchKernelGGL((attn_join_kernel<DT, HDP>), dim3((unsigned)a.kv.sequences * a.heads), dim3(256), 0, s, a);
 }
 
 template <int DT, bool F8>
-void launch_dim(const AttnArgs& a, bool pad, hipStream_t s) {
+void launch_dim(const AttnArgs& a, bool pad, bool few, hipStream_t s) {
     switch (padded(a.kv.head_dim)) {
-        case 32: return pad ? launch<DT, F8, 32, true>(a, s) : launch<DT, F8, 32, false>(a, s);
-        case 64: return pad ? launch<DT, F8, 64, true>(a, s) : launch<DT, F8, 64, false>(a, s);
-        case 128: return pad ? launch<DT, F8, 128, true>(a, s) : launch<DT, F8, 128, false>(a, s);
-        default: return pad ? launch<DT, F8, 256, true>(a, s) : launch<DT, F8, 256, false>(a, s);
+        case 32: return pad ? launch<DT, F8, 32, true>(a, few, s) : launch<DT, F8, 32, false>(a, few, s);
+        case 64: return pad ? launch<DT, F8, 64, true>(a, few, s) : launch<DT, F8, 64, false>(a, few, s);
+        case 128: return pad ? launch<DT, F8, 128, true>(a, few, s) : launch<DT, F8, 128, false>(a, few, s);
+        default: return pad ? launch<DT, F8, 256, true>(a, few, s) : launch<DT, F8, 256, false>(a, few, s);
     }
 }
 
@@ -571,8 +713,9 @@ void launch_dim(const AttnArgs& a, bool pad, hipStream_t s) {
 extern "C" int64_t hyena_attn_step_ws_bytes(const hyena_kv_pages* kv, int64_t heads) {
     if (!kv || kv->sequences <= 0 || heads <= 0 || kv->kv_heads <= 0 || kv->head_dim <= 0 || kv->head_dim > 256 || heads % kv->kv_heads)
         return 0;
+    if (short_rows(kv, heads)) return 0;
     const int64_t g = heads / kv->kv_heads, rows = g < 16 ? g : 16;
-    return 2 * (int64_t)waves_for(kv->head_dim) * rows * (padded(kv->head_dim) + 2) * 4 +
+    return 2 * waves_for(kv, heads) * rows * (padded(kv->head_dim) + 2) * 4 +
            kv->sequences * kv->kv_heads * ((g + 15) / 16) * 8;
 }
 
@@ -592,7 +735,8 @@ extern "C" int hyena_attn_step(const hyena_kv_pages* kv, const hyena_heads* q, c
     if (kv->sequences * heads >= (1LL << 31))
         return hyena_fail(HYENA_EINVAL, "%s: %lld sequences of %lld heads", who, (long long)kv->sequences, (long long)heads);
     const int64_t need = hyena_attn_step_ws_bytes(kv, heads);
-    if (!ws || ws_bytes < need || ((uintptr_t)ws & 15))
+    const bool few = short_rows(kv, heads);
+    if (!few && (!ws || ws_bytes < need || ((uintptr_t)ws & 15)))
         return hyena_fail(HYENA_EINVAL, "%s: workspace of %lld bytes (16-byte aligned), %lld needed", who, (long long)ws_bytes,
                           (long long)need);
     a.q = qh.ptr;
@@ -604,7 +748,7 @@ extern "C" int hyena_attn_step(const hyena_kv_pages* kv, const hyena_heads* q, c
     a.heads = (int32_t)heads;
     a.group = (int32_t)(heads / kv->kv_heads);
     a.qtiles = (a.group + 15) / 16;
-    a.waves = waves_for(kv->head_dim);
+    a.waves = (int32_t)waves_for(kv, heads);
     a.part_o = (float*)ws;
     a.part_ml = a.part_o + 2 * (int64_t)a.waves * (a.group < 16 ? a.group : 16) * padded(kv->head_dim);
     a.runs = (int32_t*)(a.part_ml + 4 * (int64_t)a.waves * (a.group < 16 ? a.group : 16));
@@ -614,7 +758,7 @@ extern "C" int hyena_attn_step(const hyena_kv_pages* kv, const hyena_heads* q, c
     const bool pad = kv->head_dim != padded(kv->head_dim) ||
                      (f8 && ((kv->k.page_stride | kv->k.head_stride | kv->k.slot_stride) & 15));
     hipStream_t s = (hipStream_t)stream;
-    if (dtype == HYENA_DTYPE_BF16) f8 ? launch_dim<HYENA_DTYPE_BF16, true>(a, pad, s) : launch_dim<HYENA_DTYPE_BF16, false>(a, pad, s);
-    else f8 ? launch_dim<HYENA_DTYPE_F16, true>(a, pad, s) : launch_dim<HYENA_DTYPE_F16, false>(a, pad, s);
+    if (dtype == HYENA_DTYPE_BF16) f8 ? launch_dim<HYENA_DTYPE_BF16, true>(a, pad, few, s) : launch_dim<HYENA_DTYPE_BF16, false>(a, pad, few, s);
+    else f8 ? launch_dim<HYENA_DTYPE_F16, true>(a, pad, few, s) : launch_dim<HYENA_DTYPE_F16, false>(a, pad, few, s);
     return hyena_check_launch(who);
 }
