@@ -732,6 +732,9 @@ extern "C" int hyena_attn_step(const hyena_kv_pages* kv, const hyena_heads* q, c
     if (((uintptr_t)out & 15)) return hyena_fail(HYENA_EALIGN, "%s: out must be 16-byte aligned", who);
     KvHeads qh;
     if ((rc = kv_heads_check(q, true, "q", kv->sequences, heads, &qh, who))) return rc;
+    // a lane's place in a 16-key piece is a 32-bit offset
+    if (kv->page_size > 1 && (a.kv.k.slot_stride < 0 || a.kv.v.slot_stride < 0 || a.kv.k.slot_stride > (1 << 27) || a.kv.v.slot_stride > (1 << 27)))
+        return hyena_fail(HYENA_ENOSUP, "%s: positions of a page that lie %lld bytes apart", who, (long long)a.kv.k.slot_stride);
     if (kv->sequences * heads >= (1LL << 31))
         return hyena_fail(HYENA_EINVAL, "%s: %lld sequences of %lld heads", who, (long long)kv->sequences, (long long)heads);
     const int64_t need = hyena_attn_step_ws_bytes(kv, heads);

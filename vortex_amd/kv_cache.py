@@ -239,3 +239,258 @@ def kv_copy_pages(pools, src, dst, *, dst_pools=None):
     if n:
         _enqueue("hyena_kv_copy_pages", index, a, b, pools.shape[0], size, src.data_ptr(), dst.data_ptr(), n)
     return out
+
+
+class PagedKVCache:
+    """Keys and values of a batch of sequences over all attention layers, in pages (the role of vortex/model/cache.py:8-28
+    for sequences of different lengths that come, fork and go).
+
+    pools [2*layers, pages, kv_heads, page_size, head_dim] is allocated once; pool 2i holds layer i's keys, 2i + 1 its
+    values.  A page holds `page_size` positions of one sequence in every layer.  Pages are handed out as sequences
+    grow, shared by forked sequences and copied when one of them writes into a page that others still use.  All counting
+    is on the host; table [rows, width] and lens [rows] (int32) are its device copies, which the kernels read.
+
+        cache = PagedKVCache(layers=8, kv_heads=32, head_dim=128, num_pages=4096, max_len=32768)
+        cache.add(2)                        # two empty sequences
+        pos = cache.extend([100, 37])       # room for their prompts; positions [2 * 100] of the padded batch
+        ... rotary_append(q, k, v, pos, turns, *cache.layer(i), cache.table) in every layer
+        cache.select([0, 0, 0, 1])          # the first one forked into three
+        pos = cache.extend(1)               # one more token each: the shared last page is copied for two of them
+        ... attn_step(q, *cache.layer(i), cache.table, cache.lens)
+    """
+
+    def __init__(self, layers, kv_heads, head_dim, num_pages, max_len, *, page_size=64, dtype=torch.bfloat16, fp8=False,
+                 device="cuda"):
+        if dtype not in _ACT:
+            raise TypeError(f"a cache of {dtype}: bfloat16 and float16 have kernels")
+        if page_size < 16 or page_size > 65536 or page_size & (page_size - 1):
+            raise ValueError(f"page_size {page_size} is not a power of two from 16 to 65536")
+        if head_dim % 8 or not 0 < head_dim <= 256:
+            raise ValueError(f"head_dim {head_dim} is not a multiple of 8 up to 256")
+        if min(layers, kv_heads, num_pages, max_len) < 1:
+            raise ValueError("layers, kv_heads, num_pages and max_len must be positive")
+        self.page_size, self.max_len, self.dtype, self.fp8 = page_size, max_len, dtype, fp8
+        self.width = -(-max_len // page_size)
+        self.pools = torch.empty(2 * layers, num_pages, kv_heads, page_size, head_dim,
+                                 dtype=torch.float8_e4m3fn if fp8 else dtype, device=device)
+        # per layer and side one scale a head, 1 until calibrated (e4m3 pages only)
+        self.scales = torch.ones(2 * layers, kv_heads, dtype=torch.float32, device=device) if fp8 else None
+        self._free = list(range(num_pages - 1, -1, -1))
+        self._refs = [0] * num_pages
+        self._pages, self._len = [], []         # per row: its pages in order, the positions it holds
+        self.recorded = False                   # a recorded token step uses table and lens: they stay where they are
+        self._set_rows()
+
+    @property
+    def rows(self):
+        return len(self._len)
+
+    @property
+    def free_pages(self):
+        return len(self._free)
+
+    def lengths(self):
+        """Positions that each row holds, as the host counts them."""
+        return list(self._len)
+
+    def layer(self, i):
+        """(k_pages, v_pages) of attention layer i."""
+        return self.pools[2 * i], self.pools[2 * i + 1]
+
+    def layer_scales(self, i):
+        """k_scale and v_scale of layer i as keyword arguments of rotary_append and attn_step."""
+        if self.scales is None:
+            return {}
+        return dict(k_scale=self.scales[2 * i], v_scale=self.scales[2 * i + 1])
+
+    def _set_rows(self):
+        dev = self.pools.device
+        self.table = torch.empty((self.rows, self.width), dtype=torch.int32, device=dev)
+        self.lens = torch.empty(self.rows, dtype=torch.int32, device=dev)
+        self._fill()
+
+    def _fill(self):
+        """The host's copy of the table from the lists of pages, and the device's from that."""
+        self._host = torch.full((self.rows, self.width), -1, dtype=torch.int32)
+        for row, pages in zip(self._host, self._pages):
+            row[:len(pages)] = torch.tensor(pages, dtype=torch.int32)
+        self._upload()
+
+    def _upload(self):
+        if self.rows:
+            self.table.copy_(self._host)
+            self.lens.copy_(torch.tensor(self._len, dtype=torch.int32))
+
+    def _not_recorded(self):
+        if self.recorded:
+            raise RuntimeError("a recorded token step uses this cache: release it first")
+
+    def add(self, n=1):
+        """n more empty sequences behind the others; returns the index of the first."""
+        self._not_recorded()
+        if n < 0:
+            raise ValueError(f"{n} sequences")
+        first = self.rows
+        self._pages += [[] for _ in range(n)]
+        self._len += [0] * n
+        self._set_rows()
+        return first
+
+    def select(self, rows):
+        """Keeps the named rows, in that order: one named several times is forked (its pages are shared), one not named
+        is dropped and its pages are free again."""
+        self._not_recorded()
+        rows = list(rows)
+        if any(not 0 <= r < self.rows for r in rows):
+            raise ValueError(f"rows {rows} of {self.rows}")
+        pages, lens, seen = [], [], set()
+        for r in rows:
+            mine = list(self._pages[r])
+            if r in seen:                       # pages reserved ahead stay with the first
+                mine = mine[:-(-self._len[r] // self.page_size)]
+            seen.add(r)
+            for p in mine:
+                self._refs[p] += 1
+            pages.append(mine)
+            lens.append(self._len[r])
+        for old in self._pages:
+            self._drop(old)
+        self._pages, self._len = pages, lens
+        self._set_rows()
+
+    def _drop(self, pages):
+        for p in pages:
+            self._refs[p] -= 1
+            if self._refs[p] == 0:
+                self._free.append(p)
+
+    def _give(self, counts):
+        """Pages for counts[r] more positions of every row, and own copies of shared pages that would be written to.
+        Raises, with nothing changed, where they do not fit.  Returns whether the table changed."""
+        ps, need, shared = self.page_size, 0, {}
+        for r, n in enumerate(counts):
+            if n < 0 or self._len[r] + n > self.max_len:
+                raise ValueError(f"row {r}: {n} more positions behind {self._len[r]} (at most {self.max_len})")
+            need += max(0, -(-(self._len[r] + n) // ps) - len(self._pages[r]))
+            if n and self._len[r] % ps:
+                p = self._pages[r][self._len[r] // ps]
+                if self._refs[p] - shared.get(p, 0) > 1:
+                    shared[p] = shared.get(p, 0) + 1
+                    need += 1
+        if need > len(self._free):
+            raise RuntimeError(f"{need} pages needed, {len(self._free)} of {len(self._refs)} free")
+        src, dst, changed = [], [], False
+        for r, n in enumerate(counts):
+            mine = self._pages[r]
+            if n and self._len[r] % ps:
+                at = self._len[r] // ps
+                p = mine[at]
+                if self._refs[p] > 1:
+                    mine[at] = self._host[r, at] = self._take()
+                    self._refs[p] -= 1
+                    src.append(p)
+                    dst.append(mine[at])
+                    changed = True
+            for _ in range(-(-(self._len[r] + n) // ps) - len(mine)):
+                mine.append(self._take())
+                self._host[r, len(mine) - 1] = mine[-1]
+                changed = True
+        if src:
+            self._copy(src, dst)
+        return changed
+
+    def _take(self):
+        p = self._free.pop()
+        self._refs[p] = 1
+        return p
+
+    def _copy(self, src, dst, dst_pools=None):
+        both = torch.tensor([src, dst], dtype=torch.int32, device=self.pools.device)
+        kv_copy_pages(self.pools, both[0], both[1], dst_pools=dst_pools)
+
+    def reserve(self, n):
+        """Hands out the pages of n more positions of every row ahead (an int or one count a row): extend, or a recorded
+        token step, then changes the lengths only."""
+        self._not_recorded()
+        if self._give(self._counts(n)):
+            self._upload()
+
+    def _counts(self, n):
+        counts = [n] * self.rows if isinstance(n, int) else list(n)
+        if len(counts) != self.rows:
+            raise ValueError(f"{len(counts)} counts for {self.rows} rows")
+        return counts
+
+    def extend(self, n):
+        """Makes room for n more positions of every row (an int or one count a row) and counts them as held: the call
+        ahead of a step's appends.  Returns the positions [rows * max(n)] int32 of the (padded) batch of new tokens, -1
+        where a row has fewer."""
+        self._not_recorded()
+        counts = self._counts(n)
+        most = max(counts, default=0)
+        if self._give(counts):
+            self._len = [a + b for a, b in zip(self._len, counts)]
+            self._upload()
+        else:
+            self._len = [a + b for a, b in zip(self._len, counts)]
+            if isinstance(n, int):
+                self.lens.add_(n)
+            else:
+                self.lens.copy_(torch.tensor(self._len, dtype=torch.int32))
+        if isinstance(n, int) and n == 1:
+            return self.lens - 1
+        step = torch.arange(most, dtype=torch.int32, device=self.lens.device)
+        more = self.lens.new_tensor(counts)[:, None]
+        pos = self.lens[:, None] - more + step
+        return torch.where(step < more, pos, torch.full_like(pos, -1)).reshape(-1)
+
+    def record(self, tokens):
+        """For a recorded token step (a HIP graph): hands out the pages of `tokens` more positions of every row and
+        leaves table and lens in place until release().  The step itself calls step()."""
+        self.reserve(tokens)
+        self.recorded = True
+
+    def step(self):
+        """extend(1) on the device alone, inside a recorded step: the host learns of it at release()."""
+        self.lens.add_(1)
+        return self.lens - 1
+
+    def release(self, steps):
+        """Ends record(): `steps` recorded steps have run."""
+        self.recorded = False
+        self._len = [n + steps for n in self._len]
+
+    def compact(self):
+        """Moves the pages in use to the lowest ids (one launch over all layers) and returns how many they are."""
+        self._not_recorded()
+        live = sorted(p for p in range(len(self._refs)) if self._refs[p])
+        n = len(live)
+        src = [p for p in live if p >= n]
+        dst = [p for p in range(n) if not self._refs[p]]
+        if src:
+            self._copy(src, dst)                # a page that moves is never where another one goes
+            self._rename(dict(zip(src, dst)), len(self._refs))
+        return n
+
+    def _rename(self, to, num_pages):
+        refs = [0] * num_pages
+        for p, c in enumerate(self._refs):
+            if c:
+                refs[to.get(p, p)] = c
+        self._refs = refs
+        self._free = [p for p in range(num_pages - 1, -1, -1) if not refs[p]]
+        self._pages = [[to.get(p, p) for p in pages] for pages in self._pages]
+        self._fill()
+
+    def resize(self, num_pages):
+        """Another number of pages: the ones in use are copied to the lowest ids of new pools."""
+        self._not_recorded()
+        live = sorted(p for p in range(len(self._refs)) if self._refs[p])
+        if num_pages < max(1, len(live)):
+            raise ValueError(f"{num_pages} pages for {len(live)} in use")
+        pools = torch.empty(self.pools.shape[0], num_pages, *self.pools.shape[2:], dtype=self.pools.dtype,
+                            device=self.pools.device)
+        if live:
+            self._copy(live, list(range(len(live))), dst_pools=pools)
+        self.pools = pools
+        self._rename({p: i for i, p in enumerate(live)}, num_pages)

@@ -17,6 +17,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import ops
+from .kv_cache import PagedKVCache, attn_step, rotary_append, rotary_turns
 from .cascade import (HyenaCascade, HyenaCascadeFIRInferenceParams, HyenaCascadeIIRInferenceParams,
                       project_sequence_major)
 
@@ -63,14 +64,17 @@ class GatedMLP(nn.Module):
         return torch.cat([self._f(z[:, i:i + self.chunk]) for i in range(0, z.shape[1], self.chunk)], dim=1)
 
 
-def _rotary(x, base, offset=0):
-    """x [B, L, H, hd]; non-interleaved rotary embedding over the whole head dimension."""
+def _rotary(x, base, offset=0, factor=1.0):
+    """x [B, L, H, hd]; non-interleaved rotary embedding over the whole head dimension.  factor: positions are divided by
+    it (vortex/model/model.py:77-81, rotary_emb_scaling_factor)."""
     B, L, H, hd = x.shape
     inv = 1.0 / (base ** (torch.arange(0, hd, 2, device=x.device, dtype=torch.float32) / hd))
     if isinstance(offset, torch.Tensor):            # position kept on the device (recorded token step)
         t = offset.to(torch.float32) + torch.arange(L, device=x.device, dtype=torch.float32)
     else:
         t = torch.arange(offset, offset + L, device=x.device, dtype=torch.float32)
+    if factor != 1.0:
+        t = t / factor
     f = torch.outer(t, inv)
     cos, sin = f.cos()[None, :, None].to(x.dtype), f.sin()[None, :, None].to(x.dtype)
     x1, x2 = x[..., : hd // 2], x[..., hd // 2:]
@@ -87,11 +91,35 @@ class AttentionInferenceParams:
         self.offset_dev = None      # int64 [1] device tensor while a recorded token step owns the position
 
 
+class PagedAttentionInferenceParams:
+    """Keys and values of the attention blocks in pages (kv_cache.PagedKVCache), for batches whose sequences have their
+    own lengths or share a prompt.  `slots`: the cache layer of each attention block's layer_idx."""
+
+    def __init__(self, cache, slots, turns):
+        self.cache, self.slots, self.turns = cache, slots, turns
+        self.seqlen_offset = 0      # kept by callers as for the other caches; the cache counts for itself
+        self.offset_dev = None
+        self.positions, self.first = None, False
+
+    def begin(self, batch, length):
+        """Makes room for a step's tokens; the model calls it ahead of the blocks."""
+        if batch != self.cache.rows:
+            raise ValueError(f"a batch of {batch} on a cache of {self.cache.rows} sequences")
+        if self.cache.recorded:
+            if length != 1:
+                raise RuntimeError("a recorded token step takes one token")
+            self.positions, self.first = self.cache.step(), False
+        else:
+            self.first = not any(self.cache.lengths())
+            self.positions = self.cache.extend(length)
+
+
 class AttentionBlock(nn.Module):
     def __init__(self, cfg, layer_idx):
         super().__init__()
         D, H = cfg["hidden_size"], cfg["num_attention_heads"]
         self.H, self.base, self.layer_idx = H, cfg["rotary_emb_base"], layer_idx
+        self.rotary_factor = cfg.get("rotary_emb_scaling_factor", 1.0)
         self.pre_norm, self.post_norm = RMSNorm(D, cfg["eps"]), RMSNorm(D, cfg["eps"])
         self.Wqkv = nn.Linear(D, 3 * D, bias=False)
         self.out_proj = nn.Linear(D, D, bias=True)
@@ -101,10 +129,13 @@ class AttentionBlock(nn.Module):
         B, L, D = u.shape
         hd = D // self.H
         qkv = self.Wqkv(self.pre_norm(u)).view(B, L, 3, self.H, hd)
+        if isinstance(inference_params, PagedAttentionInferenceParams):
+            return self._finish(u, self._paged_attention(qkv, inference_params))
         cached = inference_params is not None and self.layer_idx in inference_params.key_value_memory_dict
         on_device = cached and inference_params.offset_dev is not None
         off = inference_params.offset_dev if on_device else (inference_params.seqlen_offset if cached else 0)
-        q, k = _rotary(qkv[:, :, 0], self.base, off).transpose(1, 2), _rotary(qkv[:, :, 1], self.base, off).transpose(1, 2)
+        q = _rotary(qkv[:, :, 0], self.base, off, self.rotary_factor).transpose(1, 2)
+        k = _rotary(qkv[:, :, 1], self.base, off, self.rotary_factor).transpose(1, 2)
         v = qkv[:, :, 2].transpose(1, 2)                                    # [B, H, L, hd]
         if inference_params is not None and not cached:
             # zero-filled: the recorded token step reads every row (masked), and 0 * garbage could be NaN
@@ -133,8 +164,33 @@ class AttentionBlock(nn.Module):
                 o = F.scaled_dot_product_attention(q, kk, vv, attn_mask=mask)
             else:
                 o = F.scaled_dot_product_attention(q, k, v, is_causal=True)
-        u = self.out_proj(o.transpose(1, 2).reshape(B, L, D)) + u
+        return self._finish(u, o.transpose(1, 2))
+
+    def _finish(self, u, o):
+        """o [B, L, H, hd]"""
+        u = self.out_proj(o.reshape(u.shape)) + u
         return self.mlp(self.post_norm(u)) + u, None
+
+    def _paged_attention(self, qkv, ip):
+        """Rotation and append in one launch; a new token's attention over the pages in another.  A prompt on an empty
+        cache attends to itself (SDPA on the rotated rows); a longer continuation is a batch of single queries that
+        share their sequence's table row."""
+        B, L, _, H, hd = qkv.shape
+        cache, i = ip.cache, ip.slots[self.layer_idx]
+        kp, vp = cache.layer(i)
+        scales = cache.layer_scales(i)
+        q, k, v = qkv.view(B * L, 3, H, hd).unbind(1)
+        prompt = ip.first and L > 1
+        k_out = torch.empty(B * L, H, hd, dtype=k.dtype, device=k.device) if prompt else None
+        q = rotary_append(q, k, v, ip.positions, ip.turns, kp, vp, cache.table, k_out=k_out, **scales)
+        if prompt:
+            q, k, v = (x.view(B, L, H, hd).transpose(1, 2) for x in (q, k_out, v))
+            return F.scaled_dot_product_attention(q, k, v, is_causal=True).transpose(1, 2)
+        if L == 1:
+            o = attn_step(q, kp, vp, cache.table, cache.lens, **scales)
+        else:
+            o = attn_step(q, kp, vp, cache.table.repeat_interleave(L, 0), ip.positions + 1, **scales)
+        return o.view(B, L, H, hd)
 
 
 class HyenaBlock(nn.Module):
@@ -218,14 +274,56 @@ class StripedHyena2(nn.Module):
                 p.data = p.data.to(torch.bfloat16)
         return self.eval()
 
-    def initialize_inference_params(self, max_seqlen=8192):
-        """vortex/model/model.py:796-830: one cache object per operator family."""
+    def initialize_inference_params(self, max_seqlen=8192, *, kv="dense", rows=1, page_size=64, num_pages=None, fp8=False):
+        """vortex/model/model.py:796-830: one cache object per operator family.  kv="paged": the attention blocks keep
+        their keys and values in pages, num_pages of page_size positions in all (default: room for `rows` sequences of
+        max_seqlen), in 8 bits with fp8=True."""
+        if kv == "dense":
+            mha = AttentionInferenceParams(max_seqlen)
+        elif kv == "paged":
+            cfg, w = self.cfg, self.embedding.weight
+            slots = {i: n for n, i in enumerate(i for i, k in enumerate(self.kinds) if k == "attn")}
+            hd = cfg["hidden_size"] // cfg["num_attention_heads"]
+            if num_pages is None:
+                num_pages = rows * -(-max_seqlen // page_size)
+            cache = PagedKVCache(max(len(slots), 1), cfg["num_attention_heads"], hd, num_pages, max_seqlen,
+                                 page_size=page_size, dtype=w.dtype, fp8=fp8, device=w.device)
+            cache.add(rows)
+            turns = rotary_turns(hd, cfg["rotary_emb_base"], factor=cfg.get("rotary_emb_scaling_factor", 1.0), device=w.device)
+            mha = PagedAttentionInferenceParams(cache, slots, turns)
+        else:
+            raise ValueError(f"kv={kv!r}: 'dense' or 'paged'")
         return {"hcl": HyenaCascadeIIRInferenceParams(), "hcm": HyenaCascadeFIRInferenceParams(),
-                "hcs": HyenaCascadeFIRInferenceParams(), "mha": AttentionInferenceParams(max_seqlen)}
+                "hcs": HyenaCascadeFIRInferenceParams(), "mha": mha}
+
+    def select_inference_params(self, ipd, rows):
+        """Keeps the named sequences of a batch's caches, in that order: one named several times is forked, one not named
+        is dropped.  Pages of a paged cache are shared until a fork writes to them; every other cache is copied."""
+        rows = list(rows)
+        for kind, block in zip(self.kinds, self.blocks):
+            if kind == "attn":
+                continue
+            block.filter.flush_decode_state()
+            ip, i = ipd[kind], block.filter.layer_idx
+            for d in (ip.fir_state_dict, getattr(ip, "fir_inner_state_dict", {})):
+                if i in d:
+                    d[i] = d[i].select(rows)
+            if i in ip.state_dict:
+                at = torch.tensor(rows, device=ip.state_dict[i].device)
+                ip.state_dict[i] = ip.state_dict[i].index_select(0, at).contiguous()
+        mha = ipd["mha"]
+        if isinstance(mha, PagedAttentionInferenceParams):
+            mha.cache.select(rows)
+        else:
+            for i, kv in mha.key_value_memory_dict.items():
+                at = torch.tensor(rows, device=kv[0].device)
+                mha.key_value_memory_dict[i] = tuple(t.index_select(0, at) for t in kv)
 
     @torch.no_grad()
     def forward(self, input_ids, inference_params_dict=None):
         x = self.embedding(input_ids)
+        if inference_params_dict is not None and isinstance(inference_params_dict["mha"], PagedAttentionInferenceParams):
+            inference_params_dict["mha"].begin(*input_ids.shape)
         for kind, block in zip(self.kinds, self.blocks):
             ip = None if inference_params_dict is None else inference_params_dict["mha" if kind == "attn" else kind]
             x, _ = block(x, inference_params=ip)
@@ -233,15 +331,24 @@ class StripedHyena2(nn.Module):
         return x @ self.embedding.weight.T
 
     @torch.no_grad()
-    def generate(self, input_ids, num_tokens, forced=None, graph=False, window_state=True):
+    def generate(self, input_ids, num_tokens, forced=None, graph=False, window_state=True, *, kv="dense", page_size=64,
+                 fp8=False, samples=1):
         """Greedy cached generation in the order of vortex/model/generation.py:164-229: one prefill over the
         prompt, then one token per forward with the caches' seqlen_offset advanced first.  `forced`
         [B, num_tokens] replaces the sampled tokens (teacher forcing).  graph=True replays the token step as a
         recorded HIP graph from the fifth token on (RecordedDecodeStep).  window_state: the Hyena-LI layers keep their
         modal states in windows of four tokens where that form exists (HyenaCascade.window_decode_state); this loop
-        owns its caches and nobody reads them between tokens.  Returns (tokens, logits of every step)."""
+        owns its caches and nobody reads them between tokens.  kv="paged": attention keys and values in pages (in 8 bits
+        with fp8=True).  samples: continuations per prompt; the prompts are run once and their caches forked, row
+        b * samples + i of `forced` and of the results is continuation i of prompt b (several variants behind one prefix).
+        Returns (tokens, logits of every step)."""
         B, L = input_ids.shape
-        ipd = self.initialize_inference_params(max_seqlen=L + num_tokens)
+        if samples < 1:
+            raise ValueError(f"samples={samples}")
+        # forks share the full pages of their prompt
+        pages = B * (L // page_size + samples * (-(-(L + num_tokens) // page_size) - L // page_size))
+        ipd = self.initialize_inference_params(max_seqlen=L + num_tokens, kv=kv, rows=B, page_size=page_size,
+                                               num_pages=pages, fp8=fp8)
         for kind, block in zip(self.kinds, self.blocks):
             if kind != "attn":
                 block.filter.window_decode_state = window_state
@@ -252,8 +359,11 @@ class StripedHyena2(nn.Module):
                 for p in ipd.values():
                     p.seqlen_offset = L if p.seqlen_offset == 0 else p.seqlen_offset + 1
             if graph and i == 5:                    # four eager token steps have bound the decode kernels and opened
-                rec = RecordedDecodeStep(self, ipd, B)   # every window of the windowed modal steps by now
+                rec = RecordedDecodeStep(self, ipd, B * samples)   # every window of the windowed modal steps by now
             logits = (self.forward(x, ipd) if rec is None else rec(x))[:, -1]
+            if i == 0 and samples > 1:
+                self.select_inference_params(ipd, [b for b in range(B) for _ in range(samples)])
+                logits = logits.repeat_interleave(samples, 0)
             new = logits.argmax(-1) if forced is None else forced[:, i]
             toks.append(new)
             scores.append(logits)
@@ -294,17 +404,25 @@ class RecordedDecodeStep:
         if any(getattr(r, "valid", r.R) < r.R for r in rings if isinstance(r, ops.FirRing)):
             raise NotImplementedError("a cache is still filling up (prompt shorter than a filter): step eagerly")
         mha = ipd["mha"]
+        self.paged = mha.cache if isinstance(mha, PagedAttentionInferenceParams) else None
+        if self.paged is not None:              # pages for every token that fits; the positions move on the device
+            self.room = self.paged.max_len - max(self.paged.lengths())
+            self.paged.record(self.room)
         self.clock = ops.RingClock(rings)
-        mha.offset_dev = torch.tensor([mha.seqlen_offset], dtype=torch.int64, device=dev)
+        if self.paged is None:
+            mha.offset_dev = torch.tensor([mha.seqlen_offset], dtype=torch.int64, device=dev)
         self.tokens = torch.zeros(batch, 1, dtype=torch.int64, device=dev)
         self.steps = 0
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph):
             self.logits = model.forward(self.tokens, ipd)
             self.clock.advance()
-            mha.offset_dev.add_(1)
+            if self.paged is None:
+                mha.offset_dev.add_(1)
 
     def __call__(self, tokens):
+        if self.paged is not None and self.steps >= self.room:
+            raise RuntimeError(f"the paged cache has room for {self.room} recorded tokens")
         self.tokens.copy_(tokens)
         self.graph.replay()
         self.steps += 1
@@ -312,4 +430,7 @@ class RecordedDecodeStep:
 
     def release(self):
         self.clock.release()
-        self.ipd["mha"].offset_dev = None
+        if self.paged is not None:
+            self.paged.release(self.steps)
+        else:
+            self.ipd["mha"].offset_dev = None

@@ -497,6 +497,16 @@ class FirRing:
         """The slots as [B, R, D] in storage order (slot `pos` is the oldest); a view for block = D."""
         return self.buf.permute(0, 2, 1, 3).reshape(self.B, self.R, self.D)
 
+    def select(self, rows):
+        """A ring with the named rows of the batch (several times where named several times): a copy."""
+        if self.pos_dev is not None:
+            raise RuntimeError("the ring's position is on a RingClock: release it first")
+        at = torch.tensor(list(rows), device=self.buf.device)
+        ring = FirRing(self.slots().index_select(0, at), self.pos % max(self.R, 1), self.block)
+        if hasattr(self, "valid"):
+            ring.valid = self.valid
+        return ring
+
     def reference_order(self, dtype=torch.float32):
         pos = self.pos if self.pos_dev is None else int(self.pos_dev.item())
         idx = (torch.arange(self.R, device=self.buf.device) + pos) % self.R
