@@ -613,14 +613,15 @@ __global__ void __launch_bounds__(64 * short_waves<HDP>()) attn_short_kernel(Att
     }
 }
 
-// Rows that lie in several runs: the parts of one head weighted by 2^(m - max) and added in the order of the runs.
+// Rows that lie in several runs: the parts of one head weighted by 2^(m - max), every GROUPS-th added up by one group of
+// lanes, then the groups'.  All parts of a row in up to 32 runs are requested at once.
 // Sequences without a position get zeros here.
 template <int DT, int HDP>
 __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
     constexpr int VL = HDP / 4, GROUPS = 256 / VL, AHEAD = 4;       // lanes of a part, parts at a time, and in flight
     __shared__ __align__(16) float acc[GROUPS][HDP];
-    __shared__ float tot[GROUPS];
-    const int tid = threadIdx.x, lane = tid & 63, grp = tid / VL, d = tid % VL * 4;
+    __shared__ float tot[GROUPS], mx[GROUPS];
+    const int tid = threadIdx.x, grp = tid / VL, d = tid % VL * 4;
     const int32_t b = blockIdx.x / a.heads, head = blockIdx.x % a.heads, kh = head / a.group, in = head % a.group;
     const int32_t hd = a.kv.head_dim, gr = min(a.group, 16);
     typedef KvElem<DT> E;
@@ -633,11 +634,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
     }
     if (w0 == w1) return;
     auto slot = [&](int32_t w) { return (int64_t)(2 * w + (w == w0)) * gr + in % 16; };
-    float top = -INFINITY;
-    for (int32_t w = w0 + lane; w <= w1; w += 64) top = fmaxf(top, a.part_ml[slot(w) * 2]);
-    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-    const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f;
+    float m = -INFINITY, sum = 0.f;                 // of this group's parts
     f32x4 x = {0.f, 0.f, 0.f, 0.f};
     for (int32_t w = w0 + grp; w <= w1; w += GROUPS * AHEAD) {
         f32x4 v[AHEAD];
@@ -648,6 +645,13 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
             v[i] = *(const f32x4*)(a.part_o + s * HDP + d);
             pm[i] = a.part_ml[s * 2], ps[i] = a.part_ml[s * 2 + 1];
         }
+        float top = m;
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) top = w + GROUPS * i <= w1 ? fmaxf(top, pm[i]) : top;
+        const float base = top == -INFINITY ? 0.f : top, old = __builtin_amdgcn_exp2f(m - base);
+        m = top;
+        sum *= old;
+        x *= old;
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
             if (w + GROUPS * i > w1) continue;
@@ -657,12 +661,19 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
         }
     }
     *(f32x4*)&acc[grp][d] = x;
-    if (d == 0) tot[grp] = sum;
+    if (d == 0) tot[grp] = sum, mx[grp] = m;
     __syncthreads();
     if (tid >= hd) return;
-    float s = 0.f, v = 0.f;
+    float top = -INFINITY, s = 0.f, v = 0.f;
 #pragma unroll
-    for (int g = 0; g < GROUPS; ++g) s += tot[g], v += acc[g][tid];
+    for (int g = 0; g < GROUPS; ++g) top = fmaxf(top, mx[g]);
+    top = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+        const float f = __builtin_amdgcn_exp2f(mx[g] - top);
+        s += f * tot[g];
+        v += f * acc[g][tid];
+    }
     const float vs = a.kv.v.scale ? a.kv.v.scale[kh] : 1.f;
     y[tid] = E::put(s != 0.f ? v * (vs / s) : 0.f);
 }
