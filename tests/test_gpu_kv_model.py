@@ -65,6 +65,21 @@ def test_forked_continuations_match_their_own_generation(kv, graph):
     assert torch.equal(free[0], free[2]) and free.shape == (2 * S, 3)
 
 
+def test_model_refusals():
+    m = model(num_layers=4)
+    ids = tokens(2, 40)
+    ipd = m.initialize_inference_params(50, kv="paged", rows=2, page_size=16)
+    m(ids, ipd)
+    for rows in ([], [2], [-1], [0, 5]):
+        with pytest.raises(ValueError):
+            m.select_inference_params(ipd, rows)
+    for kw in (dict(fp8=True), dict(kv="other"), dict(samples=0), dict(kv="paged", page_size=20)):
+        with pytest.raises(ValueError):
+            m.generate(ids, 2, **kw)
+    with pytest.raises(TypeError):              # a model that was not brought to bfloat16
+        StripedHyena2(dict(CFG, num_layers=4), device="cuda").initialize_inference_params(50, kv="paged")
+
+
 def test_longer_continuation_on_a_paged_cache():
     m, L, n = model(pattern=("attn",), num_layers=2), 100, 37
     ids = tokens(2, L + n, 3)

@@ -164,6 +164,43 @@ def test_attention_strides_and_layouts():
     K.assert_rounds_to(same, y, slack)
 
 
+@pytest.mark.parametrize("hd,pad", [(64, 8), (128, 24), (256, 8), (32, 8), (80, 16)])
+def test_attention_8_bit_rows_at_odd_strides(hd, pad):
+    # rows hd + pad bytes apart: 8-byte multiples that are no 16-byte multiples, keys and values differently
+    lens = [129, 64, 7, 500]
+    k, v, table, ks, vs = cache(hd, lens, 2, hd, 16, BF, True)
+    q = torch.randn(4, 6, hd, generator=gen(1)).to(BF).to(DEV)
+    lt = torch.tensor(lens, dtype=torch.int32)
+    y, slack = K.attn(q, k, v, table, lt, hd ** -0.5, ks, vs)
+
+    def apart(x):
+        w = torch.zeros(x.shape[0], 2, 16, hd + pad, device=DEV).to(FP8)
+        w.view(torch.uint8)[..., :hd] = x.view(torch.uint8)
+        return w[..., :hd]
+
+    for kk, vv in ((apart(k), apart(v)), (k, apart(v)), (apart(k), v)):
+        K.assert_rounds_to(attn_step(q, kk, vv, table, lt.to(DEV), k_scale=ks, v_scale=vs), y, slack)
+
+
+def test_scales_on_pages_of_the_activations_type():
+    lens = [100, 33]
+    k, v, table, _, _ = cache(3, lens, 2, 64, 16, F16)
+    ks, vs = torch.tensor([0.5, 3.0], device=DEV), torch.tensor([0.125, 7.0], device=DEV)
+    q = torch.randn(2, 4, 64, generator=gen(1)).to(F16).to(DEV)
+    lt = torch.tensor(lens, dtype=torch.int32)
+    y, slack = K.attn(q, k, v, table, lt, 0.125, ks, vs)
+    K.assert_rounds_to(attn_step(q, k, v, table, lt.to(DEV), k_scale=ks, v_scale=vs), y, slack)
+    x = torch.randn(1, 2, 64, generator=gen(2)).to(F16).to(DEV)
+    kp, vp = torch.zeros(1, 2, 16, 64, dtype=F16, device=DEV), torch.zeros(1, 2, 16, 64, dtype=F16, device=DEV)
+    rotary_append(x, x, x, torch.tensor([5], dtype=torch.int32, device=DEV), rotary_turns(64, device=DEV), kp, vp,
+                  torch.zeros(1, 1, dtype=torch.int32, device=DEV), k_scale=ks, v_scale=vs)
+    w = x.double().cpu() / vs.double().cpu()[None, :, None]
+    K.assert_rounds_to(vp[:, :, 5], w, w.abs() * 2.0 ** -24)
+    w, sl = K.rotate(x, torch.tensor([5]), rotary_turns(64), False)
+    d = ks.double().cpu()[None, :, None]
+    K.assert_rounds_to(kp[:, :, 5], w / d, sl / d + (w / d).abs() * 2.0 ** -24)
+
+
 def test_attention_leaves_out_pages_that_are_not_there():
     lens = [100, 64, 40, 500]
     k, v, table, _, _ = cache(10, lens, 1, 64, 16, BF)

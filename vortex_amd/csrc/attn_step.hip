@@ -299,6 +299,7 @@ struct Walk {
     __device__ __forceinline__ void turn(int s, const u32x4 (&rows)[CPR / 4 ? CPR / 4 : 1]) {
 #pragma unroll
         for (int i = 0; i < CPR / 4; ++i) *(u32x4*)(lds + s % 2 * 16 * RB + i * 1024 + lane * 16) = rows[i];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");     // no instruction; other lanes read this
     }
     // The values of a tile, 8 bytes a lane: elements 8 * (lane % 16) .. of rows 4 * (lane / 16) + 0..3 of every piece.
     __device__ __forceinline__ void turn_values() {
@@ -768,9 +769,10 @@ extern "C" int hyena_attn_step(const hyena_kv_pages* kv, const hyena_heads* q, c
     a.runs = (int32_t*)(a.part_ml + 4 * (int64_t)a.waves * (a.group < 16 ? a.group : 16));
     const bool f8 = kv->dtype == HYENA_DTYPE_F8E4M3;
     // the plain form loads 16 bytes of a row at a time and whole rows; other row lengths and, in 8 bits, strides that
-    // are only 8-byte multiples take the form that masks the pieces behind a row's end
+    // are only 8-byte multiples take the form that loads 8 bytes and masks the pieces behind a row's end
     const bool pad = kv->head_dim != padded(kv->head_dim) ||
-                     (f8 && ((kv->k.page_stride | kv->k.head_stride | kv->k.slot_stride) & 15));
+                     (f8 && ((kv->k.page_stride | kv->k.head_stride | kv->k.slot_stride | kv->v.page_stride | kv->v.head_stride |
+                              kv->v.slot_stride) & 15));
     hipStream_t s = (hipStream_t)stream;
     if (dtype == HYENA_DTYPE_BF16) f8 ? launch_dim<HYENA_DTYPE_BF16, true>(a, pad, few, s) : launch_dim<HYENA_DTYPE_BF16, false>(a, pad, few, s);
     else f8 ? launch_dim<HYENA_DTYPE_F16, true>(a, pad, few, s) : launch_dim<HYENA_DTYPE_F16, false>(a, pad, few, s);

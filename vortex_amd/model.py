@@ -279,6 +279,8 @@ class StripedHyena2(nn.Module):
         their keys and values in pages, num_pages of page_size positions in all (default: room for `rows` sequences of
         max_seqlen), in 8 bits with fp8=True."""
         if kv == "dense":
+            if fp8:
+                raise ValueError("8-bit keys and values are kept in pages: kv='paged'")
             mha = AttentionInferenceParams(max_seqlen)
         elif kv == "paged":
             cfg, w = self.cfg, self.embedding.weight
@@ -299,7 +301,14 @@ class StripedHyena2(nn.Module):
     def select_inference_params(self, ipd, rows):
         """Keeps the named sequences of a batch's caches, in that order: one named several times is forked, one not named
         is dropped.  Pages of a paged cache are shared until a fork writes to them; every other cache is copied."""
-        rows = list(rows)
+        rows, mha = list(rows), ipd["mha"]
+        sizes = {r.B for kind in ("hcs", "hcm", "hcl") for r in ipd[kind].fir_state_dict.values()}
+        if isinstance(mha, PagedAttentionInferenceParams):
+            sizes.add(mha.cache.rows)
+        else:
+            sizes |= {kv[0].shape[0] for kv in mha.key_value_memory_dict.values()}
+        if not rows or len(sizes) != 1 or any(not 0 <= r < min(sizes) for r in rows):
+            raise ValueError(f"rows {rows} of caches that hold {sorted(sizes)} sequences")
         for kind, block in zip(self.kinds, self.blocks):
             if kind == "attn":
                 continue
@@ -311,7 +320,6 @@ class StripedHyena2(nn.Module):
             if i in ip.state_dict:
                 at = torch.tensor(rows, device=ip.state_dict[i].device)
                 ip.state_dict[i] = ip.state_dict[i].index_select(0, at).contiguous()
-        mha = ipd["mha"]
         if isinstance(mha, PagedAttentionInferenceParams):
             mha.cache.select(rows)
         else:
@@ -414,11 +422,15 @@ class RecordedDecodeStep:
         self.tokens = torch.zeros(batch, 1, dtype=torch.int64, device=dev)
         self.steps = 0
         self.graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.graph):
-            self.logits = model.forward(self.tokens, ipd)
-            self.clock.advance()
-            if self.paged is None:
-                mha.offset_dev.add_(1)
+        try:
+            with torch.cuda.graph(self.graph):
+                self.logits = model.forward(self.tokens, ipd)
+                self.clock.advance()
+                if self.paged is None:
+                    mha.offset_dev.add_(1)
+        except BaseException:
+            self.release()
+            raise
 
     def __call__(self, tokens):
         if self.paged is not None and self.steps >= self.room:

@@ -501,7 +501,10 @@ class FirRing:
         """A ring with the named rows of the batch (several times where named several times): a copy."""
         if self.pos_dev is not None:
             raise RuntimeError("the ring's position is on a RingClock: release it first")
-        at = torch.tensor(list(rows), device=self.buf.device)
+        rows = list(rows)
+        if any(not 0 <= r < self.B for r in rows):
+            raise ValueError(f"rows {rows} of a cache of {self.B}")
+        at = torch.tensor(rows, dtype=torch.int64, device=self.buf.device)
         ring = FirRing(self.slots().index_select(0, at), self.pos % max(self.R, 1), self.block)
         if hasattr(self, "valid"):
             ring.valid = self.valid
