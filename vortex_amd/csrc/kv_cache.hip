@@ -247,27 +247,29 @@ __global__ void __launch_bounds__(APPEND_THREADS) rotary_append_kernel(AppendArg
     }
 }
 
-constexpr int64_t COPY_PIECE = 16384;       // bytes of a block: four 16-byte requests a thread, all before the first store
-
-// One block per (pair, piece of the page, pool).  Bound by its bytes; non-temporal accesses, since nothing here is read
-// twice: 200 pages of 128 KB in 16 pools 163 -> 155 us (5.4 TB/s read and written), a fork into 7 5.4 -> 4.6 us.
+// One block per (pair, piece of the page, pool), N 16-byte requests a thread, all before the first store.  Bound by its
+// bytes; non-temporal accesses, since nothing here is read twice.  N = 1 streams fastest (200 pages of 128 KB in 16
+// pools: 135 us, 6.2 TB/s read and written, against 154 with N = 4), N = 4 needs fewer blocks where little is copied (a
+// fork of one such page into 7: 4.6 against 5.5 us).
+template <int N>
 __global__ void __launch_bounds__(256) copy_pages_kernel(const char* src_base, int64_t src_pool, int64_t src_page, int64_t src_pages,
                                                          char* dst_base, int64_t dst_pool, int64_t dst_page, int64_t dst_pages,
                                                          int64_t bytes, int32_t pieces, const int32_t* src, const int32_t* dst,
                                                          int wide) {
+    constexpr int64_t PIECE = 4096 * N;
     const int32_t pair = blockIdx.x / pieces, piece = blockIdx.x % pieces;
     const int64_t s = src[pair], d = dst[pair];
     if (s < 0 || s >= src_pages || d < 0 || d >= dst_pages) return;
-    const char* from = src_base + (int64_t)blockIdx.y * src_pool + s * src_page + piece * COPY_PIECE;
-    char* to = dst_base + (int64_t)blockIdx.y * dst_pool + d * dst_page + piece * COPY_PIECE;
-    const int64_t n = min(COPY_PIECE, bytes - piece * COPY_PIECE);
+    const char* from = src_base + (int64_t)blockIdx.y * src_pool + s * src_page + piece * PIECE;
+    char* to = dst_base + (int64_t)blockIdx.y * dst_pool + d * dst_page + piece * PIECE;
+    const int64_t n = min(PIECE, bytes - piece * PIECE);
     const int tid = threadIdx.x;
-    if (wide && n == COPY_PIECE) {
-        u32x4 x[4];
+    if (wide && n == PIECE) {
+        u32x4 x[N];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = __builtin_nontemporal_load((const u32x4*)from + tid + 256 * i);
+        for (int i = 0; i < N; ++i) x[i] = __builtin_nontemporal_load((const u32x4*)from + tid + 256 * i);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) __builtin_nontemporal_store(x[i], (u32x4*)to + tid + 256 * i);
+        for (int i = 0; i < N; ++i) __builtin_nontemporal_store(x[i], (u32x4*)to + tid + 256 * i);
         return;
     }
     const int64_t n16 = wide ? n / 16 : 0;
@@ -379,13 +381,14 @@ extern "C" int hyena_kv_copy_pages(const hyena_kv_pools* src_pools, const hyena_
     const int64_t at = (int64_t)((uintptr_t)src_pools->base | (uintptr_t)dst_pools->base) |
                        (pools > 1 ? src_pools->pool_stride | dst_pools->pool_stride : 0) | src_pools->page_stride | dst_pools->page_stride;
     const int wide = (at & 15) == 0;
-    const int64_t pieces = (page_bytes + COPY_PIECE - 1) / COPY_PIECE;
+    const bool much = copies * pools > (64 << 20) / page_bytes;
+    const int64_t piece = much ? 4096 : 16384, pieces = (page_bytes + piece - 1) / piece;
     if (copies * pieces >= (1LL << 31))
         return hyena_fail(HYENA_EINVAL, "%s: %lld copies of %lld bytes are too many for one call", who, (long long)copies,
                           (long long)page_bytes);
-    hipLaunchKernelGGL(copy_pages_kernel, dim3((unsigned)(copies * pieces), (unsigned)pools), dim3(256), 0, (hipStream_t)stream,
-                       (const char*)src_pools->base, src_pools->pool_stride, src_pools->page_stride, src_pools->pages,
-                       (char*)dst_pools->base, dst_pools->pool_stride, dst_pools->page_stride, dst_pools->pages, page_bytes,
-                       (int32_t)pieces, src, dst, wide);
+    hipLaunchKernelGGL(much ? copy_pages_kernel<1> : copy_pages_kernel<4>, dim3((unsigned)(copies * pieces), (unsigned)pools),
+                       dim3(256), 0, (hipStream_t)stream, (const char*)src_pools->base, src_pools->pool_stride,
+                       src_pools->page_stride, src_pools->pages, (char*)dst_pools->base, dst_pools->pool_stride,
+                       dst_pools->page_stride, dst_pools->pages, page_bytes, (int32_t)pieces, src, dst, wide);
     return hyena_check_launch(who);
 }
