@@ -26,14 +26,16 @@ _HEADS = struct.Struct("@P2q").pack
 _POOLS = struct.Struct("@P3q").pack
 
 
-# torch.cuda.current_stream builds a Stream object; this returns its handle
+# torch.cuda.current_stream builds a Stream object and current_device checks for initialisation (tensors of the device
+# exist here); these return the handle and the index
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _enqueue(name, index, *args):
     """Calls an entry point on the current stream of device `index`, which is made current for the call."""
     fn = getattr(_lib.lib(), name)
-    if index == torch.cuda.current_device():
+    if index == _current_device():
         rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
@@ -95,12 +97,12 @@ def _kv(k_pages, v_pages, table, k_scale, v_scale, act):
 
 
 def _head_rows(t, name, shape, dtype):
+    st = t.stride()
     if t.dtype is not dtype:
         raise TypeError(f"{name} is {t.dtype}, expected {dtype}")
-    ts, hs, one = t.stride() if t.dim() == 3 else (0, 0, 0)
-    if t.shape != shape or (one != 1 and shape[2] > 1):
+    if t.shape != shape or (st[2] != 1 and shape[2] > 1):
         raise ValueError(f"{name} must be {list(shape)} with contiguous head_dim, got {tuple(t.shape)}")
-    return _HEADS(t.data_ptr(), ts, hs)
+    return _HEADS(t.data_ptr(), st[0], st[1])
 
 
 def rotary_turns(rotary_dim, base=10000.0, *, factor=1.0, scaling="linear", original_length=None, slow_turns=1.0,
