@@ -65,6 +65,13 @@ def test_forked_continuations_match_their_own_generation(kv, graph):
     assert torch.equal(free[0], free[2]) and free.shape == (2 * S, 3)
 
 
+def test_a_stack_without_attention_takes_the_paged_keyword():
+    m, ids = model(pattern=("hcs", "hcm", "hcl"), num_layers=3), tokens(2, 150)
+    _, want = m.generate(ids, 8, forced=ids[:, :8])
+    _, got = m.generate(ids, 8, forced=ids[:, :8], kv="paged", graph=True)
+    assert torch.equal(got, want)
+
+
 def test_model_refusals():
     m = model(num_layers=4)
     ids = tokens(2, 40)

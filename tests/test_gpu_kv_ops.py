@@ -134,6 +134,64 @@ def test_attention_infinities():
     assert float(got[3, 0, 7]) == float("inf") and bool(got[3, 0, :7].isfinite().all())
 
 
+def test_attention_small_weights_count_what_they_are():
+    # bf16: a value of 1e30 behind a weight of 2^-115 (or one that underflows) must not come through; f16: one weight of
+    # 1 and 20000 of 2^-12 that together outweigh it
+    k, v, table, _, _ = cache(12, [300, 300], 1, 64, 16, BF)
+    q = torch.zeros(2, 1, 64, dtype=BF, device=DEV)
+    q[:, 0, 0] = 1.0
+    k[..., 0] = 0.0
+    for b, low in ((0, -79.5), (1, -200.0)):
+        p = table[b, 7].item()
+        k[p, 0, 3], v[p, 0, 3] = 0.0, 1e30
+        k[p, 0, 3, 0] = low
+    check_attn(q, (k, v, table, None, None), [300, 300], 1.0)
+    n = 20000
+    k, v, table, _, _ = cache(13, [n], 1, 64, 64, F16)
+    k[...] = 0.0
+    k[table[0, 100].item(), 0, 9, 0] = 8.3125
+    v.copy_((v.float().nan_to_num().abs() + 0.5).to(F16))
+    q = torch.zeros(1, 1, 64, dtype=F16, device=DEV)
+    q[0, 0, 0] = 1.0
+    lt = torch.tensor([n], dtype=torch.int32)
+    y, slack = K.attn(q, k, v, table, lt, 1.0)
+    # terms are kept to 2^-35 of the largest weight here, and a sum's rounding errors do not all point one way: half of
+    # the general slack's 2^-16 and (2 n + 128) 2^-24 terms is ample, and its 2^-25 term does not apply
+    slack = y.abs() * (2.0 ** -15 + 2.0 ** -13) / 2 + n * 2.0 ** -35 * v.float().nan_to_num().abs().max().item() / (1 + n * 2.0 ** -12)
+    K.assert_rounds_to(attn_step(q, k, v, table, lt.to(DEV), scale=1.0), y, slack)
+
+
+def test_attention_heads_do_not_touch_each_other():
+    # NaN or infinities in one query head, and in a shared value column, stay there
+    lens, H = [200, 33], 6
+    c = cache(14, lens, 2, 64, 16, BF)
+    q = torch.randn(2, H, 64, generator=gen(5)).to(BF).to(DEV)
+    lt = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    want = attn_step(q, *c[:3], lt)
+    for bad in (float("nan"), float("inf")):
+        x = q.clone()
+        x[0, 4, 3] = bad
+        got = attn_step(x, *c[:3], lt)
+        keep = torch.ones(2, H, dtype=torch.bool, device=DEV)
+        keep[0, 4] = False
+        assert torch.equal(got[keep], want[keep]) and bool(got[0, 4].isnan().all())
+    c[1][c[2][0, 2].item(), 1, 3, 5] = float("nan")
+    got = attn_step(q, *c[:3], lt)
+    assert bool(got[0, 3:, 5].isnan().all())
+    got[0, 3:, 5] = want[0, 3:, 5]
+    assert torch.equal(got, want)
+
+
+def test_attention_many_sequences_and_large_pages():
+    r = torch.randint(0, 5, (1500,), generator=gen(15)).tolist()
+    c = cache(15, r, 1, 32, 16, BF)
+    check_attn(torch.randn(1500, 2, 32, generator=gen(6)).to(BF).to(DEV), c, r)
+    for page, hd in ((65536, 8), (4096, 64)):
+        lens = [70000, 3] if page > 60000 else [5000, 4097, 4096]
+        c = cache(16, lens, 1, hd, page, BF, spare=1)
+        check_attn(torch.randn(len(lens), 1, hd, generator=gen(7)).to(BF).to(DEV), c, lens)
+
+
 def test_attention_strides_and_layouts():
     lens, kv_heads, group, hd, page = [129, 64, 7], 2, 3, 64, 32
     k, v, table, _, _ = cache(9, lens, kv_heads, hd, page, BF)

@@ -19,7 +19,6 @@
 namespace {
 
 constexpr int WAVES = 4;                    // wavefronts of a block (they share nothing)
-constexpr float LAZY = 8.f;                 // the maximum follows the scores when one exceeds it by more than 2^8
 constexpr int64_t STREAM_BYTES = 128 << 20; // reads beyond this are non-temporal
 
 struct AttnArgs {
@@ -36,23 +35,28 @@ struct AttnArgs {
     int32_t waves;                          // of the even cut
 };
 
+// Weights are 2^(score - m + SHIFT), m a running maximum that follows the scores when one exceeds it by more than
+// LAZY.  float16 needs the shift: it brings the largest weights to 2^15 and with them the smallest terms a weight is
+// kept in (2^-24) to 2^-35 of the largest.
 template <int DT> struct Mma;
 template <> struct Mma<HYENA_DTYPE_BF16> {
+    static constexpr float LAZY = 8.f, SHIFT = 0.f;
     static __device__ __forceinline__ f32x4 dot(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
     static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf2(lo, hi); }
     // weights x, y >= 0 as head (cut off, not rounded) + rest; the rest is never 0, so that a weight times an
-    // infinite value stays infinite instead of adding 0 * inf
+    // infinite value stays infinite instead of adding 0 * inf; it is the least that float32 weights go down to
     static __device__ __forceinline__ void split(float x, float y, uint32_t& head, uint32_t& rest) {
         head = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
-        rest = pack(fmaxf(x - bf_lo(head), 0x1p-100f), fmaxf(y - bf_hi(head), 0x1p-100f));
+        rest = pack(fmaxf(x - bf_lo(head), 0x1p-126f), fmaxf(y - bf_hi(head), 0x1p-126f));
     }
     template <bool HI> static __device__ __forceinline__ uint32_t from_f8(uint32_t w) {
         return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, HI));
     }
 };
 template <> struct Mma<HYENA_DTYPE_F16> {
+    static constexpr float LAZY = 4.f, SHIFT = 11.f;
     typedef __attribute__((__vector_size__(2 * sizeof(_Float16)))) _Float16 h2;
     static __device__ __forceinline__ f32x4 dot(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -406,7 +410,7 @@ struct Walk {
             for (int i = 0; i < 2 * NT; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) top = fmaxf(top, s[i][e]);
-            if (__any(top > m + LAZY)) {                // the maximum moves for all heads of the tile at once
+            if (__any(top > m + M::LAZY)) {                // the maximum moves for all heads of the tile at once
                 const float mn = fmaxf(m, max_over_keys(top)), f = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
                 m = mn;
                 l *= f;
@@ -414,7 +418,7 @@ struct Walk {
 #pragma unroll
                 for (int i = 0; i < VB * DL; ++i) o[i] *= g;
             }
-            const float base = m == -INFINITY ? 0.f : m;
+            const float base = m == -INFINITY ? 0.f : m - M::SHIFT;
 #pragma unroll
             for (int i = 0; i < 2 * NT; ++i)
 #pragma unroll
