@@ -7,6 +7,8 @@
 //   hyena_fir_step_far                the same step on a deep cache read whole only every third token, 3 ring periods
 //   hyena_iir_step                    one modal update against the closed form
 //   hyena_iir_step_win                the modal step with the state in windows of tokens against hyena_iir_step (float32 rounding)
+//   hyena_rotary_append, hyena_attn_step, hyena_kv_copy_pages
+//                                     a quarter turn written into a page, equal scores give the mean value, a page copied
 //   argument errors                   negative return codes and a message
 // Usage: abi_selftest /path/to/libhyena_mi355x.so
 #include <dlfcn.h>
@@ -50,6 +52,7 @@ int main(int argc, char** argv) {
     SYM(hyena_iir_step_win) SYM(hyena_iir_window_flush) SYM(hyena_iir_window_tokens) SYM(hyena_iir_window_supported)
     SYM(hyena_fir_layer_fwd_rows) SYM(hyena_li_layer_fwd) SYM(hyena_li_fwd) SYM(hyena_li_plan) SYM(hyena_li_plan_bytes)
     SYM(hyena_set_launch_override)
+    SYM(hyena_rotary_append) SYM(hyena_attn_step) SYM(hyena_attn_step_ws_bytes) SYM(hyena_kv_copy_pages)
     printf("%s\n", p_hyena_version());
     hipStream_t stream; HIP_OK(hipStreamCreate(&stream));
 
@@ -358,6 +361,71 @@ int main(int argc, char** argv) {
         }
         flush_and_compare(10);
         printf("hyena_iir_step_win / hyena_iir_window_flush (windows of %lld tokens) against hyena_iir_step: ok\n", (long long)W);
+    }
+
+    // ---- paged key / value cache: two sequences, pages of 16 positions, 2 query heads on one key head of 64
+    {
+        const int64_t hd = 64, ps = 16, P = 5, S = 2, H = 2, T = 6;     // three tokens a sequence
+        std::vector<uint16_t> q(T * H * hd), k(T * hd), v(T * hd), zero(P * ps * hd, 0);
+        for (int64_t t = 0; t < T; ++t)
+            for (int64_t d = 0; d < hd; ++d) {
+                k[t * hd + d] = to_bf16((float)(t + 1) * (d < 32 ? 1.f : 0.5f));
+                v[t * hd + d] = to_bf16((float)(4 * t + d % 4));
+                for (int64_t h = 0; h < H; ++h) q[(t * H + h) * hd + d] = to_bf16(d < 32 ? 2.f : -1.f);
+            }
+        std::vector<int32_t> table = {3, 1, 4, -1}, pos = {14, 15, 16, 0, 1, 2}, lens = {17, 3};
+        std::vector<double> turns(hd / 2, 0.25);                        // position p: p quarter turns
+        uint16_t *dq = dev(q), *dk = dev(k), *dv = dev(v), *kp = dev(zero), *vp = dev(zero), *qo = dev(q), *out = dev(q);
+        int32_t *d_table = dev(table), *d_pos = dev(pos), *d_lens = dev(lens);
+        double* d_turns = dev(turns);
+        hyena_kv_pages kv = {};
+        kv.k = {kp, ps * hd, ps * hd, hd, nullptr};
+        kv.v = {vp, ps * hd, ps * hd, hd, nullptr};
+        kv.num_pages = P, kv.page_size = ps, kv.kv_heads = 1, kv.head_dim = hd;
+        kv.table = d_table, kv.table_stride = 2, kv.table_width = 2, kv.sequences = S, kv.dtype = HYENA_DTYPE_BF16;
+        hyena_heads hq = {dq, H * hd, hd}, hk = {dk, hd, hd}, hv = {dv, hd, hd}, ho = {qo, H * hd, hd};
+        int rc = p_hyena_rotary_append(&kv, &hq, &hk, &hv, &ho, nullptr, d_pos, nullptr, d_turns, hd, 0, 0, T, H,
+                                       HYENA_DTYPE_BF16, stream);
+        CHECK(rc == 0, "hyena_rotary_append rc=%d: %s", rc, p_hyena_last_error_string());
+        HIP_OK(hipStreamSynchronize(stream));
+        auto pk = host(kp, zero.size()); auto pv = host(vp, zero.size()); auto pq = host(qo, q.size());
+        const int64_t at[6] = {3 * ps + 14, 3 * ps + 15, 1 * ps, 4 * ps, 4 * ps + 1, 4 * ps + 2};
+        for (int64_t t = 0; t < T; ++t) {
+            const int quarter = pos[t] % 4;
+            const float c[4] = {1, 0, -1, 0}, sn[4] = {0, 1, 0, -1};
+            for (int64_t d = 0; d < 32; ++d) {
+                const float x1 = (float)(t + 1), x2 = 0.5f * (t + 1);
+                CHECK(from_bf16(pk[at[t] * hd + d]) == x1 * c[quarter] - x2 * sn[quarter] &&
+                          from_bf16(pk[at[t] * hd + 32 + d]) == x1 * sn[quarter] + x2 * c[quarter], "rotated key t=%d d=%d", (int)t, (int)d);
+                CHECK(pv[at[t] * hd + d] == v[t * hd + d], "value t=%d d=%d", (int)t, (int)d);
+                CHECK(from_bf16(pq[t * H * hd + d]) == 2.f * c[quarter] + sn[quarter], "rotated query t=%d d=%d", (int)t, (int)d);
+            }
+        }
+        // scale 0: every position weighs the same; sequence 0 sees 14 zero values ahead of its three, sequence 1 its three
+        const int64_t nws = p_hyena_attn_step_ws_bytes(&kv, H);
+        void* ws; HIP_OK(hipMalloc(&ws, nws + 16));
+        hyena_heads h2 = {qo, H * hd, hd};
+        rc = p_hyena_attn_step(&kv, &h2, d_lens, 0.f, out, ws, nws, H, HYENA_DTYPE_BF16, stream);
+        CHECK(rc == 0, "hyena_attn_step rc=%d: %s", rc, p_hyena_last_error_string());
+        HIP_OK(hipStreamSynchronize(stream));
+        auto o = host(out, (size_t)(S * H * hd));
+        for (int64_t s = 0; s < S; ++s)
+            for (int64_t i = 0; i < H * hd; ++i) {
+                const int64_t d = i % hd;
+                const float want = s == 0 ? (float)(12 + 3 * (d % 4)) / 17.f : (float)(48 + 3 * (d % 4)) / 3.f;
+                CHECK(fabsf(from_bf16(o[s * H * hd + i]) - want) <= want / 256.f, "mean value s=%d i=%d got %g want %g", (int)s,
+                      (int)i, from_bf16(o[s * H * hd + i]), want);
+            }
+        std::vector<int32_t> src = {3}, dst = {0};
+        int32_t *d_src = dev(src), *d_dst = dev(dst);
+        hyena_kv_pools pools = {vp, P * ps * hd * 2, ps * hd * 2, P};
+        rc = p_hyena_kv_copy_pages(&pools, &pools, 1, ps * hd * 2, d_src, d_dst, 1, stream);
+        CHECK(rc == 0, "hyena_kv_copy_pages rc=%d: %s", rc, p_hyena_last_error_string());
+        HIP_OK(hipStreamSynchronize(stream));
+        auto pc = host(vp, zero.size());
+        CHECK(memcmp(pc.data(), pc.data() + 3 * ps * hd, ps * hd * 2) == 0 && memcmp(pc.data() + ps * hd, pv.data() + ps * hd, 4 * ps * hd * 2) == 0,
+              "copied page");
+        printf("hyena_rotary_append / hyena_attn_step / hyena_kv_copy_pages on pages: ok\n");
     }
 
     // ---- rejected arguments come back as negative codes with a message, before anything is launched

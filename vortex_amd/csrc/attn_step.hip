@@ -76,10 +76,6 @@ template <> struct Mma<HYENA_DTYPE_F16> {
 };
 
 __device__ __forceinline__ int lane_id() { return __lane_id(); }
-__device__ __forceinline__ int64_t uniform(int64_t x) {
-    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x), hi = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32));
-    return (int64_t)(((uint64_t)hi << 32) | lo);
-}
 __device__ __forceinline__ float max_over_keys(float x) {       // over the four lanes lane, lane ^ 16, ^ 32, ^ 48
     x = fmaxf(x, __shfl_xor(x, 16));
     return fmaxf(x, __shfl_xor(x, 32));

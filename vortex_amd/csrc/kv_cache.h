@@ -7,7 +7,6 @@ typedef __attribute__((__vector_size__(8 * sizeof(_Float16)))) _Float16 f16x8;
 template <int DT> struct KvElem;            // a stored or an activation element as float32, and back
 template <> struct KvElem<HYENA_DTYPE_BF16> {
     typedef uint16_t raw;
-    static __device__ __forceinline__ float get(raw r) { return bf_to_f(r); }
     static __device__ __forceinline__ raw put(float f) { return (raw)f_to_bf_bits(f); }
     static __device__ __forceinline__ float lo(uint32_t w) { return bf_lo(w); }
     static __device__ __forceinline__ float hi(uint32_t w) { return bf_hi(w); }
@@ -22,15 +21,12 @@ template <> struct KvElem<HYENA_DTYPE_F16> {
     static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return put(lo) | (uint32_t)put(hi) << 16; }
 };
 template <> struct KvElem<HYENA_DTYPE_F8E4M3> {
-    typedef uint8_t raw;
-    static __device__ __forceinline__ float get(raw r) { return __builtin_amdgcn_cvt_f32_fp8((int)r, 0); }
     // round to nearest even; the instruction turns what lies beyond +-448 into NaN, so the value is clamped first
     // (NaN compares false both times and stays)
     static __device__ __forceinline__ float clamp(float f) { return f > 448.f ? 448.f : (f < -448.f ? -448.f : f); }
     static __device__ __forceinline__ uint32_t pack(float a, float b) {         // two values in the low 16 bits
         return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(clamp(a), clamp(b), 0, false) & 0xffffu;
     }
-    static __device__ __forceinline__ raw put(float f) { return (raw)pack(f, 0.f); }
 };
 
 struct KvSide {
