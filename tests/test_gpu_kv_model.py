@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from oracle import kv_oracle as KO
 from vortex_amd import PagedKVCache, attn_step, rotary_append, rotary_turns
 from vortex_amd.model import EVO2_7B, RecordedDecodeStep, StripedHyena2
 
@@ -87,8 +88,30 @@ def test_model_refusals():
         StripedHyena2(dict(CFG, num_layers=4), device="cuda").initialize_inference_params(50, kv="paged")
 
 
-def test_longer_continuation_on_a_paged_cache():
-    m, L, n = model(pattern=("attn",), num_layers=2), 100, 37
+@pytest.mark.parametrize("fp8", [False, True])
+def test_dense_rows_of_a_paged_cache(fp8):
+    c = PagedKVCache(2, 3, 40, 12, 100, page_size=16, fp8=fp8)
+    c.add(3)
+    c.extend([50, 0, 17])
+    c.pools.copy_(torch.randn(c.pools.shape, device="cuda").mul(4).to(c.pools.dtype))
+    c.pools[:, c._free] = float("nan")                      # free pages, and a page's slots behind its sequence's end
+    c.pools[:, c._pages[0][3], :, 2:] = float("nan")
+    if fp8:
+        c.scales.copy_(0.1 + torch.rand(c.scales.shape, device="cuda"))
+    for side, x in enumerate(c.dense(1)):
+        assert x.shape == (3, 3, 50, 40) and x.dtype == torch.bfloat16
+        for r, n in enumerate(c.lengths()):
+            assert not x[r, :, n:].any()
+            for p in range(n):
+                want = c.pools[2 + side, c._pages[r][p // 16], :, p % 16].double()
+                if fp8:
+                    want = want * c.scales[2 + side].double()[:, None]
+                KO.assert_rounds_to(x[r, :, p], want.cpu(), want.abs().cpu() * 2.0 ** -24)
+
+
+@pytest.mark.parametrize("n", [2, 32, 33, 60])
+def test_longer_continuation_on_a_paged_cache(n):
+    m, L = model(pattern=("attn",), num_layers=2), 100
     ids = tokens(2, L + n, 3)
     want = m(ids)[:, L:]
     ipd = m.initialize_inference_params(L + n, kv="paged", rows=2, page_size=16)

@@ -305,6 +305,23 @@ class PagedKVCache:
             return {}
         return dict(k_scale=self.scales[2 * i], v_scale=self.scales[2 * i + 1])
 
+    def dense(self, i):
+        """Keys and values of layer i as two [rows, kv_heads, max(lengths), head_dim] tensors of the activations' type,
+        zero behind a row's end: for attention of many new tokens at once, where reading the pages once into rows is
+        cheaper than reading them for every token."""
+        n = max(self._len, default=0)
+        w = -(-n // self.page_size)
+        at = self.table[:, :w].clamp(min=0).long()
+        behind = torch.arange(w * self.page_size, device=self.lens.device) >= self.lens[:, None]
+        out = []
+        for s, pages in enumerate(self.layer(i)):
+            x = pages.view(torch.uint8)[at].view(pages.dtype) if self.fp8 else pages[at]         # [rows, w, heads, size, hd]
+            x = x.permute(0, 2, 1, 3, 4).reshape(self.rows, pages.shape[1], w * self.page_size, pages.shape[3])
+            if self.fp8:
+                x = (x.float() * self.scales[2 * i + s][:, None, None]).to(self.dtype)
+            out.append(x.masked_fill(behind[:, None, :, None], 0)[:, :, :n])
+        return tuple(out)
+
     def _set_rows(self):
         dev = self.pools.device
         self.table = torch.empty((self.rows, self.width), dtype=torch.int32, device=dev)

@@ -30,6 +30,9 @@ EVO2_7B = dict(
 )
 
 
+# New tokens of a continuation that attn_step takes one by one; more read the pages once into rows (32 heads of 128 behind
+# 8192 positions: 16 tokens 0.20 against 0.68 ms, 64 tokens 1.17 against 0.74).
+PAGED_QUERIES = 32
 SEQ_MAJOR = "auto"      # "never": every Hyena block hands its operator a channel-last projection
 
 
@@ -173,8 +176,8 @@ class AttentionBlock(nn.Module):
 
     def _paged_attention(self, qkv, ip):
         """Rotation and append in one launch; a new token's attention over the pages in another.  A prompt on an empty
-        cache attends to itself (SDPA on the rotated rows); a longer continuation is a batch of single queries that
-        share their sequence's table row."""
+        cache attends to itself (SDPA on the rotated rows); a continuation of a few tokens is a batch of single queries
+        that share their sequence's table row, a longer one gathers the pages and runs SDPA."""
         B, L, _, H, hd = qkv.shape
         cache, i = ip.cache, ip.slots[self.layer_idx]
         kp, vp = cache.layer(i)
@@ -188,8 +191,12 @@ class AttentionBlock(nn.Module):
             return F.scaled_dot_product_attention(q, k, v, is_causal=True).transpose(1, 2)
         if L == 1:
             o = attn_step(q, kp, vp, cache.table, cache.lens, **scales)
-        else:
+        elif L <= PAGED_QUERIES:
             o = attn_step(q, kp, vp, cache.table.repeat_interleave(L, 0), ip.positions + 1, **scales)
+        else:
+            k, v = cache.dense(i)
+            seen = torch.arange(k.shape[2], device=q.device) <= ip.positions.view(B, 1, L, 1)
+            return F.scaled_dot_product_attention(q.view(B, L, H, hd).transpose(1, 2), k, v, attn_mask=seen).transpose(1, 2)
         return o.view(B, L, H, hd)
 
 
