@@ -451,16 +451,17 @@ int hyena_fir_layer_fwd(const hyena_proj_fwd* proj,
 /* ---- Paged key / value cache of the attention blocks -------------------------------------------------------------
  *
  * The reference's attention blocks keep one [B, max_seqlen, 2, H, head_dim] tensor per layer (vortex/model/cache.py:8-28)
- * or a paged cache addressed through a block table (vortex/ops/attn_interface.py, flash_attn_with_kvcache).  Here a
- * layer's cache is pages of `page_size` positions: element (page, head, slot, d) of a side sits at
+ * or a paged cache addressed through a block table (vortex/ops/attn_interface.py).  Here a layer's cache is pages of
+ * `page_size` positions: element (page, head, slot, d) of a side sits at
  *   ptr + page*page_stride + head*head_stride + slot*slot_stride + d         (strides in elements, d contiguous),
  * and position j of sequence s lives in page table[s*table_stride + j / page_size], slot j % page_size.
  * `scale` [kv_heads] float32 (or NULL for 1): what a stored value is multiplied by; e4m3 pages use it.
  * A page id outside 0..num_pages-1 names no page: nothing is read from or written to it (attention leaves its positions
  * out, an append drops them), and so do positions beyond table_width*page_size.
  * Rules (others: HYENA_ENOSUP / HYENA_EALIGN): head_dim a multiple of 8 up to 256; page_size a power of two from 16 to
- * 65536; a table row names at most 2^30 positions; strides multiples of 8 elements (that of a dimension of one element is not looked at), pointers 16-byte
- * aligned. */
+ * 65536; a table row names at most 2^30 positions; strides multiples of 8 elements (that of a dimension of one element
+ * is not looked at), pointers 16-byte aligned; in attention the positions of a page lie at most 2^27 bytes apart; an
+ * append takes at most 32768 heads, whose rows for 16 tokens lie within 2^32 bytes. */
 typedef struct hyena_kv_side {
     void* ptr;
     int64_t page_stride, head_stride, slot_stride;
@@ -483,12 +484,13 @@ typedef struct hyena_heads {
 } hyena_heads;
 
 /* Attention of ONE new token per sequence over its cached positions 0..lens[s]-1 (the token's own key among them: append
- * first).  Replaces the cached single-token branch of vortex/model/attention.py (flash_attn_with_kvcache / the
- * non-flash products :247-283).  For head h of sequence s, with g = heads / kv_heads:
+ * first).  Replaces the cached single-token branch of vortex/model/attention.py (the products of :247-283).  For head h
+ * of sequence s, with g = heads / kv_heads:
  *   w_j = exp(scale * k.scale[h/g] * <q, K_j> - max),  out = v.scale[h/g] * sum_j w_j V_j / sum_j w_j
  * q [sequences][heads][head_dim] (token_stride = sequence stride), out the same, contiguous, of the type of q (`dtype`:
- * BF16 or F16).  lens[s] <= 0 gives zeros; lens[s] beyond the table's reach counts as its reach.  Values behind
- * lens[s] in a page may be anything, NaN included.  Sums and softmax statistics are float32.
+ * BF16 or F16).  lens[s] <= 0 gives zeros, and so does a sequence none of whose positions has a page or a score above
+ * -inf; lens[s] beyond the table's reach counts as its reach.  Values behind lens[s] in a page may be anything, NaN
+ * included.  Sums and softmax statistics are float32; results do not depend on timing.
  * ws: hyena_attn_step_ws_bytes(kv, heads) bytes of device memory (16-byte aligned; may be 0) for the parts of long
  * sequences, contents of no interest before and after; calls that overlap in time need one each. */
 int64_t hyena_attn_step_ws_bytes(const hyena_kv_pages* kv, int64_t heads);
