@@ -282,11 +282,13 @@ def test_c_entry_points_refuse_before_launching():
                      (EINVAL, app(qo=None)), (EINVAL, app(pos=None)), (EINVAL, app(turns=None)), (EINVAL, app(rd=63)),
                      (EINVAL, app(rd=66)), (EINVAL, app(rd=-2)), (EINVAL, app(T=-1)), (EINVAL, app(T=5)), (EINVAL, app(H=0)),
                      (ENOSUP, app(H=40000)), (EALIGN, app(q=heads(4104))), (EALIGN, app(ko=heads(head=12))), (ENOSUP, app(dt=2)),
+                     (EINVAL, app(qo=heads(tok=0))), (EINVAL, app(ko=heads(head=0))), (EINVAL, app(kv=pages(strides=(0, 1024, 64)))),
+                     (EINVAL, app(kv=pages(strides=(4096, 0, 64)))), (EINVAL, app(kv=pages(strides=(4096, 1024, 0)))),
                      (ENOSUP, app(q=heads(tok=1 << 28))), (ENOSUP, app(k=heads(head=-64))), (0, app(T=0))]:
         assert rc == want, L.hyena_last_error_string()
     pool = lambda base=P, ps=4096, n=5: kv_cache._POOLS(base, 1 << 20, ps, n)
     copy = lambda a=pool(), b=pool(), n=2, size=64, s=P, d=P, c=3: L.hyena_kv_copy_pages(a, b, n, size, s, d, c, None)
     for want, rc in [(EINVAL, copy(a=None)), (EINVAL, copy(b=pool(base=0))), (EINVAL, copy(s=None)), (EINVAL, copy(n=-1)),
                      (EINVAL, copy(n=70000)), (EINVAL, copy(c=-1)), (EINVAL, copy(c=1 << 31)), (EINVAL, copy(size=-4)),
-                     (EINVAL, copy(c=1 << 30, size=1 << 20)), (0, copy(c=0)), (0, copy(n=0)), (0, copy(size=0))]:
+                     (EINVAL, copy(c=1 << 30, size=1 << 20)), (EINVAL, copy(b=pool(ps=0))), (0, copy(c=0)), (0, copy(n=0)), (0, copy(size=0))]:
         assert rc == want, L.hyena_last_error_string()

@@ -345,9 +345,14 @@ extern "C" int hyena_rotary_append(const hyena_kv_pages* kv, const hyena_heads* 
             if (h->token_stride < 0 || h->head_stride < 0 || APPEND_TOKENS * h->token_stride + n * h->head_stride >= (1LL << 32))
                 return hyena_fail(HYENA_ENOSUP, "%s: rows of %s that lie %lld bytes apart", who, in_name[i],
                                   (long long)h->token_stride);
+        if (r.dst.ptr && ((tokens > 1 && r.dst.token_stride == 0) || (n > 1 && r.dst.head_stride == 0)))
+            return hyena_fail(HYENA_EINVAL, "%s: rows of %s share their memory", who, to_name[i]);
         r.heads = (uint32_t)n;
         r.magic = n == 1 ? 0 : (uint32_t)(((1ULL << 32) + n - 1) / n);
     }
+    for (const hyena_kv_side* side : {&kv->k, &kv->v})
+        if ((kv->num_pages > 1 && side->page_stride == 0) || (kv->kv_heads > 1 && side->head_stride == 0) || side->slot_stride == 0)
+            return hyena_fail(HYENA_EINVAL, "%s: positions of the pages share their memory", who);
     if (!pos || (rotary_dim > 0 && !turns)) return hyena_fail(HYENA_EINVAL, "%s: pos and turns are required", who);
     if (rotary_dim < 0 || rotary_dim % 2 || rotary_dim > kv->head_dim)
         return hyena_fail(HYENA_EINVAL, "%s: rotary_dim %lld is not an even number up to head_dim %lld", who,
@@ -380,6 +385,8 @@ extern "C" int hyena_kv_copy_pages(const hyena_kv_pools* src_pools, const hyena_
     if (pools == 0 || copies == 0 || page_bytes == 0) return 0;
     if (!src_pools->base || !dst_pools->base || !src || !dst)
         return hyena_fail(HYENA_EINVAL, "%s: pools, src and dst are required", who);
+    if ((pools > 1 && dst_pools->pool_stride == 0) || (dst_pools->pages > 1 && dst_pools->page_stride == 0))
+        return hyena_fail(HYENA_EINVAL, "%s: destination pages share their memory", who);
     const int64_t at = (int64_t)((uintptr_t)src_pools->base | (uintptr_t)dst_pools->base) |
                        (pools > 1 ? src_pools->pool_stride | dst_pools->pool_stride : 0) | src_pools->page_stride | dst_pools->page_stride;
     const int wide = (at & 15) == 0;
