@@ -97,45 +97,51 @@ __device__ __forceinline__ int32_t seq_len(const AttnArgs& a, int32_t b) {
     return (int32_t)min((int64_t)max(a.lens[b], 0), a.kv.reach);
 }
 
-__device__ __forceinline__ uint32_t scan64(uint32_t x, int lane) {          // inclusive, over the lanes
+__device__ __forceinline__ int64_t scan64(int64_t x, int lane) {            // inclusive, over the lanes
     for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t up = __shfl_up(x, o);
+        const int64_t up = __shfl_up(x, o);
         x += lane >= o ? up : 0;
     }
     return x;
 }
+__device__ __forceinline__ int64_t of_lane(int64_t x, int lane) {
+    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)x, lane), hi = __builtin_amdgcn_readlane((uint32_t)(x >> 32), lane);
+    return (int64_t)(((uint64_t)hi << 32) | lo);
+}
 
-// Sums the tiles of all sequences, 64 lengths at a time, and finds the sequence that holds the first tile of wavefront
-// w.  (The tiles of 64 sequences fit 32 bits: kv_pages_check bounds what a table row can name.)
+// Sums the tiles of all sequences, each lane those of consecutive ones, and finds the sequence that holds the first
+// tile of wavefront w: its lane first, then among that lane's.
 __device__ __forceinline__ Place find_place(const AttnArgs& a, int tk_shift, int32_t rows, int64_t w) {
     const int lane = lane_id();
+    const int64_t B = a.kv.sequences, per = (B + 63) / 64;
+    auto tiles = [&](int64_t b) { return b < B ? ((int64_t)seq_len(a, (int32_t)b) + (1 << tk_shift) - 1) >> tk_shift : 0; };
     Place p = {0, 0, 0, 0, 0};
-    const int32_t B = a.kv.sequences;
-    uint32_t mine = 0, incl = 0;
-    for (int32_t b0 = 0; b0 < B; b0 += 64) {
-        mine = b0 + lane < B ? (uint32_t)(((int64_t)seq_len(a, b0 + lane) + (1 << tk_shift) - 1) >> tk_shift) : 0;
-        incl = scan64(mine, lane);
-        p.total += (uint32_t)__builtin_amdgcn_readlane(incl, 63);
-    }
-    p.total *= rows;
+    int64_t mine = 0;
+    for (int64_t i = 0; i < per; ++i) mine += tiles(lane * per + i);
+    const int64_t incl = scan64(mine, lane);
+    p.total = of_lane(incl, 63) * rows;
     p.waves = min(p.total, (int64_t)a.waves);
     if (w >= p.waves) return p;
     const int64_t goal = kv_first_tile(w, p.total, p.waves);
-    int64_t ahead = 0;                                                      // in tiles per (key head, query tile)
-    for (int32_t b0 = 0; b0 < B; b0 += 64) {
-        if (B > 64) {
-            mine = b0 + lane < B ? (uint32_t)(((int64_t)seq_len(a, b0 + lane) + (1 << tk_shift) - 1) >> tk_shift) : 0;
-            incl = scan64(mine, lane);
-        }
-        const uint64_t hit = __ballot((ahead + incl) * rows > goal);
+    const int l = __builtin_ctzll(__ballot(incl * rows > goal));
+    int64_t ahead = of_lane(incl, l) - of_lane(mine, l);                    // in tiles per (key head, query tile)
+    if (per == 1) {
+        p.b = l;
+        p.tiles = (int32_t)of_lane(mine, l);
+        p.first = ahead * rows;
+        return p;
+    }
+    for (int64_t i = 0; i < per; i += 64) {
+        const int64_t t = i + lane < per ? tiles(l * per + i + lane) : 0, sum = scan64(t, lane);
+        const uint64_t hit = __ballot((ahead + sum) * rows > goal);
         if (hit) {
-            const int l = __builtin_ctzll(hit);
-            p.b = b0 + l;
-            p.tiles = __builtin_amdgcn_readlane(mine, l);
-            p.first = (ahead + (uint32_t)__builtin_amdgcn_readlane(incl, l) - p.tiles) * rows;
+            const int k = __builtin_ctzll(hit);
+            p.b = (int32_t)(l * per + i + k);
+            p.tiles = (int32_t)of_lane(t, k);
+            p.first = (ahead + of_lane(sum, k) - p.tiles) * rows;
             return p;
         }
-        ahead += (uint32_t)__builtin_amdgcn_readlane(incl, 63);
+        ahead += of_lane(sum, 63);
     }
     return p;
 }
@@ -619,29 +625,29 @@ __global__ void __launch_bounds__(64 * short_waves<HDP>()) attn_short_kernel(Att
 }
 
 // Rows that lie in several runs: the parts of one head weighted by 2^(m - max), every GROUPS-th added up by one group of
-// lanes, then the groups'.  All parts of a row in up to 32 runs are requested at once.
-// Sequences without a position get zeros here.
-template <int DT, int HDP>
+// lanes, then the groups'.  THREADS work on one head and request up to 32 (256 threads, heads of 128) of its parts at
+// once.  Sequences without a position get zeros here.
+template <int DT, int HDP, int THREADS>
 __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
-    constexpr int VL = HDP / 4, GROUPS = 256 / VL, AHEAD = 4;       // lanes of a part, parts at a time, and in flight
-    __shared__ __align__(16) float acc[GROUPS][HDP];
-    __shared__ float tot[GROUPS], mx[GROUPS];
-    const int tid = threadIdx.x, grp = tid / VL, d = tid % VL * 4;
-    const int32_t b = blockIdx.x / a.heads, head = blockIdx.x % a.heads, kh = head / a.group, in = head % a.group;
-    const int32_t hd = a.kv.head_dim, gr = min(a.group, 16);
+    constexpr int VL = HDP / 4, GROUPS = THREADS / VL, AHEAD = 4;   // lanes of a part, parts at a time, and in flight
+    __shared__ __align__(16) float acc[256 / THREADS][GROUPS][HDP];
+    __shared__ float tot[256 / THREADS][GROUPS], mx[256 / THREADS][GROUPS];
+    const int sub = threadIdx.x / THREADS, tid = threadIdx.x % THREADS, grp = tid / VL, d = tid % VL * 4;
+    const int64_t item = (int64_t)blockIdx.x * (256 / THREADS) + sub;
+    const bool there = item < (int64_t)a.kv.sequences * a.heads;
+    const int32_t b = there ? (int32_t)(item / a.heads) : 0, head = there ? (int32_t)(item % a.heads) : 0;
+    const int32_t kh = head / a.group, in = head % a.group, hd = a.kv.head_dim, gr = min(a.group, 16);
     typedef KvElem<DT> E;
     typename E::raw* y = (typename E::raw*)a.out + ((int64_t)b * a.heads + head) * hd;
     const int32_t* run = a.runs + (((int64_t)b * a.kv.kv_heads + kh) * a.qtiles + in / 16) * 2;
     const int32_t n = seq_len(a, b), w0 = run[0], w1 = run[1];
-    if (n == 0) {
-        if (tid < hd) y[tid] = 0;
-        return;
-    }
-    if (w0 == w1) return;
+    if (there && n == 0)
+        for (int i = tid; i < hd; i += THREADS) y[i] = 0;
+    const bool join = there && n > 0 && w0 < w1;
     auto slot = [&](int32_t w) { return (int64_t)(2 * w + (w == w0)) * gr + in % 16; };
     float m = -INFINITY, sum = 0.f;                 // of this group's parts
     f32x4 x = {0.f, 0.f, 0.f, 0.f};
-    for (int32_t w = w0 + grp; w <= w1; w += GROUPS * AHEAD) {
+    for (int32_t w = w0 + grp; join && w <= w1; w += GROUPS * AHEAD) {
         f32x4 v[AHEAD];
         float pm[AHEAD], ps[AHEAD];
 #pragma unroll
@@ -665,22 +671,29 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
             x += v[i] * f;
         }
     }
-    *(f32x4*)&acc[grp][d] = x;
-    if (d == 0) tot[grp] = sum, mx[grp] = m;
+    if (join) {
+        *(f32x4*)&acc[sub][grp][d] = x;
+        if (d == 0) tot[sub][grp] = sum, mx[sub][grp] = m;
+    }
     __syncthreads();
-    if (tid >= hd) return;
-    float top = -INFINITY, s = 0.f, v = 0.f;
+    if (!join) return;
+    float top = -INFINITY, s = 0.f;
 #pragma unroll
-    for (int g = 0; g < GROUPS; ++g) top = fmaxf(top, mx[g]);
+    for (int g = 0; g < GROUPS; ++g) top = fmaxf(top, mx[sub][g]);
     top = top == -INFINITY ? 0.f : top;
+    float f[GROUPS];
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g) {
-        const float f = __builtin_amdgcn_exp2f(mx[g] - top);
-        s += f * tot[g];
-        v += f * acc[g][tid];
+        f[g] = __builtin_amdgcn_exp2f(mx[sub][g] - top);
+        s += f[g] * tot[sub][g];
     }
-    const float vs = a.kv.v.scale ? a.kv.v.scale[kh] : 1.f;
-    y[tid] = E::put(s != 0.f ? v * (vs / s) : 0.f);
+    const float vs = a.kv.v.scale ? a.kv.v.scale[kh] : 1.f, inv = s != 0.f ? vs / s : 0.f;
+    for (int i = tid; i < hd; i += THREADS) {
+        float v = 0.f;
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) v += f[g] * acc[sub][g][i];
+        y[i] = E::put(v * inv);
+    }
 }
 
 int padded(int64_t hd) { return hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
@@ -712,7 +725,11 @@ void launch(const AttnArgs& a, bool few, hipStream_t s) {
         return;
     }
     hipLaunchKernelGGL((attn_walk_kernel<DT, F8, HDP, PAD>), dim3(a.waves / WAVES), dim3(64 * WAVES), 0, s, a);
-    hipLaunchKernelGGL((attn_join_kernel<DT, HDP>), dim3((unsigned)a.kv.sequences * a.heads), dim3(256), 0, s, a);
+    // many heads have few parts each: one wavefront a head instead of a block (2048 sequences of 32
+    // keys, 32 heads: 123 -> 79 us with the walk)
+    const int64_t heads = (int64_t)a.kv.sequences * a.heads;
+    if (heads > 1024) hipLaunchKernelGGL((attn_join_kernel<DT, HDP, 64>), dim3((unsigned)((heads + 3) / 4)), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((attn_join_kernel<DT, HDP, 256>), dim3((unsigned)heads), dim3(256), 0, s, a);
 }
 
 template <int DT, bool F8>
