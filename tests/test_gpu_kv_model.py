@@ -81,7 +81,7 @@ def test_model_refusals():
     for rows in ([], [2], [-1], [0, 5]):
         with pytest.raises(ValueError):
             m.select_inference_params(ipd, rows)
-    for kw in (dict(fp8=True), dict(kv="other"), dict(samples=0), dict(kv="paged", page_size=20)):
+    for kw in (dict(fp8=True), dict(kv="other"), dict(samples=0), dict(kv="paged", page_size=20), dict(kv="paged", page_size=0)):
         with pytest.raises(ValueError):
             m.generate(ids, 2, **kw)
     with pytest.raises(TypeError):              # a model that was not brought to bfloat16
@@ -141,8 +141,9 @@ def test_selected_sequences_go_on():
                 assert cache.compact() == 2 * 7 and cache.free_pages == 7
             if i == 4:
                 rec = RecordedDecodeStep(m, ipd, 2)
-                with pytest.raises(RuntimeError, match="recorded"):
-                    cache.compact()
+                for call in (cache.compact, lambda: m.select_inference_params(ipd, [0, 0])):
+                    with pytest.raises(RuntimeError, match="recorded"):
+                        call()
             if i == 6:
                 rec.release()
                 rec = None
@@ -150,6 +151,22 @@ def test_selected_sequences_go_on():
             x = ids[rows, L + i - 1:L + i]
             got = (m(x, ipd) if rec is None else rec(x))[:, -1]
             near(got, want[rows, i])
+
+
+def test_a_recording_that_finds_no_pages_leaves_the_caches_usable():
+    m, L, n = model(), 200, 6
+    ids = tokens(2, L + n, 4)
+    _, want = m.generate(ids[:, :L], n, forced=ids[:, L:])
+    with torch.no_grad():
+        ipd = m.initialize_inference_params(4 * L, kv="paged", rows=2, page_size=16, num_pages=2 * 14)
+        m(ids[:, :L], ipd)
+        for i in range(1, n):
+            for p in ipd.values():
+                p.seqlen_offset = L if p.seqlen_offset == 0 else p.seqlen_offset + 1
+            if i == 3:
+                with pytest.raises(RuntimeError, match="pages needed"):
+                    RecordedDecodeStep(m, ipd, 2)
+            near(m(ids[:, L + i - 1:L + i], ipd)[:, -1], want[:, i])
 
 
 def test_two_recorded_caches_in_turn_and_at_once():

@@ -269,7 +269,7 @@ class PagedKVCache:
             raise ValueError(f"page_size {page_size} is not a power of two from 16 to 65536")
         if head_dim % 8 or not 0 < head_dim <= 256:
             raise ValueError(f"head_dim {head_dim} is not a multiple of 8 up to 256")
-        if min(layers, kv_heads, num_pages, max_len) < 1:
+        if min(layers, kv_heads, num_pages or 0, max_len) < 1:
             raise ValueError("layers, kv_heads, num_pages and max_len must be positive")
         self.page_size, self.max_len, self.dtype, self.fp8 = page_size, max_len, dtype, fp8
         self.width = -(-max_len // page_size)

@@ -293,7 +293,7 @@ class StripedHyena2(nn.Module):
             cfg, w = self.cfg, self.embedding.weight
             slots = {i: n for n, i in enumerate(i for i, k in enumerate(self.kinds) if k == "attn")}
             hd = cfg["hidden_size"] // cfg["num_attention_heads"]
-            if num_pages is None:
+            if num_pages is None and page_size > 0:
                 num_pages = rows * -(-max_seqlen // page_size)
             cache = PagedKVCache(max(len(slots), 1), cfg["num_attention_heads"], hd, num_pages, max_seqlen,
                                  page_size=page_size, dtype=w.dtype, fp8=fp8, device=w.device)
@@ -316,18 +316,21 @@ class StripedHyena2(nn.Module):
             sizes |= {kv[0].shape[0] for kv in mha.key_value_memory_dict.values()}
         if not rows or len(sizes) != 1 or any(not 0 <= r < min(sizes) for r in rows):
             raise ValueError(f"rows {rows} of caches that hold {sorted(sizes)} sequences")
-        for kind, block in zip(self.kinds, self.blocks):
-            if kind == "attn":
-                continue
-            block.filter.flush_decode_state()
-            ip, i = ipd[kind], block.filter.layer_idx
+        paged = isinstance(mha, PagedAttentionInferenceParams)
+        if (mha.cache.recorded if paged else mha.offset_dev is not None):
+            raise RuntimeError("a recorded token step uses these caches: release it first")
+        hyena = [(ipd[kind], block.filter) for kind, block in zip(self.kinds, self.blocks) if kind != "attn"]
+        for _, f in hyena:                      # what can be refused comes before anything moves
+            f.flush_decode_state()
+        for ip, f in hyena:
+            i = f.layer_idx
             for d in (ip.fir_state_dict, getattr(ip, "fir_inner_state_dict", {})):
                 if i in d:
                     d[i] = d[i].select(rows)
             if i in ip.state_dict:
                 at = torch.tensor(rows, device=ip.state_dict[i].device)
                 ip.state_dict[i] = ip.state_dict[i].index_select(0, at).contiguous()
-        if isinstance(mha, PagedAttentionInferenceParams):
+        if paged:
             mha.cache.select(rows)
         else:
             for i, kv in mha.key_value_memory_dict.items():
@@ -360,8 +363,9 @@ class StripedHyena2(nn.Module):
         B, L = input_ids.shape
         if samples < 1:
             raise ValueError(f"samples={samples}")
-        # forks share the full pages of their prompt
-        pages = B * (L // page_size + samples * (-(-(L + num_tokens) // page_size) - L // page_size))
+        pages = None
+        if kv == "paged" and page_size > 0:     # forks share the full pages of their prompt
+            pages = B * (L // page_size + samples * (-(-(L + num_tokens) // page_size) - L // page_size))
         ipd = self.initialize_inference_params(max_seqlen=L + num_tokens, kv=kv, rows=B, page_size=page_size,
                                                num_pages=pages, fp8=fp8)
         for kind, block in zip(self.kinds, self.blocks):
@@ -420,16 +424,16 @@ class RecordedDecodeStep:
             raise NotImplementedError("a cache is still filling up (prompt shorter than a filter): step eagerly")
         mha = ipd["mha"]
         self.paged = mha.cache if isinstance(mha, PagedAttentionInferenceParams) else None
-        if self.paged is not None:              # pages for every token that fits; the positions move on the device
-            self.room = self.paged.max_len - max(self.paged.lengths())
-            self.paged.record(self.room)
         self.clock = ops.RingClock(rings)
-        if self.paged is None:
-            mha.offset_dev = torch.tensor([mha.seqlen_offset], dtype=torch.int64, device=dev)
-        self.tokens = torch.zeros(batch, 1, dtype=torch.int64, device=dev)
         self.steps = 0
-        self.graph = torch.cuda.CUDAGraph()
         try:
+            if self.paged is not None:          # pages for every token that fits; the positions move on the device
+                self.room = self.paged.max_len - max(self.paged.lengths())
+                self.paged.record(self.room)
+            else:
+                mha.offset_dev = torch.tensor([mha.seqlen_offset], dtype=torch.int64, device=dev)
+            self.tokens = torch.zeros(batch, 1, dtype=torch.int64, device=dev)
+            self.graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(self.graph):
                 self.logits = model.forward(self.tokens, ipd)
                 self.clock.advance()
