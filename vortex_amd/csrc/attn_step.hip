@@ -11,8 +11,9 @@
 //     So the weights never move between lanes;
 //   * O = P V: a lane loads 8 consecutive elements of a value row for each of its 8 keys (full rows per 16 lanes) and
 //     pairs the keys up with one v_perm per two elements.
-// The weights go in as two 16-bit terms (16 bits of mantissa): the products are free beside the loads, and the output
-// then differs from the float32 formula by the last rounding only.
+// The weights go in as three 16-bit terms that hold all 24 bits of a float32 weight: the products are free beside the
+// loads, and what is left between the output and the float32 formula is the order of the sums (with two terms, 16 bits in
+// bf16, about one output in 2000 came out as a neighbour of the value it rounds to).
 #include "kv_addr.h"
 #include "kv_cache.h"
 
@@ -45,11 +46,19 @@ template <> struct Mma<HYENA_DTYPE_BF16> {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
     static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf2(lo, hi); }
-    // weights x, y >= 0 as head (cut off, not rounded) + rest; the rest is never 0, so that a weight times an
-    // infinite value stays infinite instead of adding 0 * inf; it is the least that float32 weights go down to
-    static __device__ __forceinline__ void split(float x, float y, uint32_t& head, uint32_t& rest) {
-        head = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
-        rest = pack(fmaxf(x - bf_lo(head), 0x1p-126f), fmaxf(y - bf_hi(head), 0x1p-126f));
+    // Weights x, y >= 0 as the exact sum of three terms, none of them 0, so that a weight times an infinite value stays
+    // infinite instead of adding 0 * inf.  A term is the largest bf16 number BELOW what is left (its predecessor cut off),
+    // which leaves 1..2^16 and then 1..2^8 units of the weight's last place.  A weight of 0 counts as the least that
+    // float32 weights go down to.
+    static __device__ __forceinline__ uint32_t below(float x, float y) {
+        return __builtin_amdgcn_perm(__float_as_uint(y) - 1, __float_as_uint(x) - 1, 0x07060302u);
+    }
+    static __device__ __forceinline__ void split(float x, float y, uint32_t (&t)[3]) {
+        x = fmaxf(x, 0x1p-126f), y = fmaxf(y, 0x1p-126f);
+        t[0] = below(x, y);
+        x -= bf_lo(t[0]), y -= bf_hi(t[0]);
+        t[1] = below(x, y);
+        t[2] = pack(x - bf_lo(t[1]), y - bf_hi(t[1]));
     }
     template <bool HI> static __device__ __forceinline__ uint32_t from_f8(uint32_t w) {
         return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, HI));
@@ -65,10 +74,14 @@ template <> struct Mma<HYENA_DTYPE_F16> {
         const h2 h = {(_Float16)lo, (_Float16)hi};
         return __builtin_bit_cast(uint32_t, h);
     }
-    static __device__ __forceinline__ void split(float x, float y, uint32_t& head, uint32_t& rest) {
-        const auto h = __builtin_amdgcn_cvt_pkrtz(x, y);
-        head = __builtin_bit_cast(uint32_t, h);
-        rest = pack(fmaxf(x - (float)h[0], 0x1p-24f), fmaxf(y - (float)h[1], 0x1p-24f));
+    // head, rest and rest of the rest, cut off and the last one rounded: all bits of a weight down to 2^-24.  The
+    // smaller two are never 0.
+    static __device__ __forceinline__ void split(float x, float y, uint32_t (&t)[3]) {
+        const auto a = __builtin_amdgcn_cvt_pkrtz(x, y);
+        x = fmaxf(x - (float)a[0], 0x1p-24f), y = fmaxf(y - (float)a[1], 0x1p-24f);
+        const auto b = __builtin_amdgcn_cvt_pkrtz(x, y);
+        t[0] = __builtin_bit_cast(uint32_t, a), t[1] = __builtin_bit_cast(uint32_t, b);
+        t[2] = pack(fmaxf(x - (float)b[0], 0x1p-24f), fmaxf(y - (float)b[1], 0x1p-24f));
     }
     template <bool HI> static __device__ __forceinline__ uint32_t from_f8(uint32_t w) {
         return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, HI));
@@ -430,14 +443,12 @@ struct Walk {
                 }
 #pragma unroll
             for (int g = 0; g < NT; ++g) {
-                u32x4 ph, pl;
+                u32x4 p[3];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float x = s[2 * g + e / 2][2 * (e % 2)], y = s[2 * g + e / 2][2 * (e % 2) + 1];
-                    uint32_t head, rest;
-                    M::split(x, y, head, rest);
-                    ph[e] = head;
-                    pl[e] = rest;
+                    uint32_t t[3];
+                    M::split(s[2 * g + e / 2][2 * (e % 2)], s[2 * g + e / 2][2 * (e % 2) + 1], t);
+                    p[0][e] = t[0], p[1][e] = t[1], p[2][e] = t[2];
                 }
 #pragma unroll
                 for (int b = 0; b < VB; ++b)
@@ -455,8 +466,8 @@ struct Walk {
                                                              i % 2 ? 0x07060302u : 0x05040100u);
                             }
                         }
-                        o[b * DL + i] = M::dot(ph, x, o[b * DL + i]);
-                        o[b * DL + i] = M::dot(pl, x, o[b * DL + i]);
+#pragma unroll
+                        for (int t = 0; t < 3; ++t) o[b * DL + i] = M::dot(p[t], x, o[b * DL + i]);
                     }
             }
             load_values<STREAM>();
