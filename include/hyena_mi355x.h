@@ -490,7 +490,8 @@ typedef struct hyena_heads {
  * q [sequences][heads][head_dim] (token_stride = sequence stride), out the same, contiguous, of the type of q (`dtype`:
  * BF16 or F16).  lens[s] <= 0 gives zeros, and so does a sequence none of whose positions has a page or a score above
  * -inf; lens[s] beyond the table's reach counts as its reach.  Values behind lens[s] in a page may be anything, NaN
- * included.  Sums and softmax statistics are float32; results do not depend on timing.
+ * included.  Sums, weights and softmax statistics are float32 (a weight below 2^-126 of the largest is 0; 0 times a value
+ * that is not finite is NaN, as in the formula); results do not depend on timing.
  * ws: hyena_attn_step_ws_bytes(kv, heads) bytes of device memory (16-byte aligned; may be 0) for the parts of long
  * sequences, contents of no interest before and after; calls that overlap in time need one each. */
 int64_t hyena_attn_step_ws_bytes(const hyena_kv_pages* kv, int64_t heads);

@@ -36,25 +36,26 @@ struct AttnArgs {
     int32_t waves;                          // of the even cut
 };
 
-// Weights are 2^(score - m + SHIFT), m a running maximum that follows the scores when one exceeds it by more than
-// LAZY.  float16 needs the shift: it brings the largest weights to 2^15 and with them the smallest terms a weight is
-// kept in (2^-24) to 2^-35 of the largest.
+// Weights are 2^(score - m + SHIFT), m a whole number that follows the scores up when one exceeds it by more than LAZY, so
+// that changing m scales the sums without a rounding.  float16 terms end at 2^-24, 2^-35 of a weight at m.  There m
+// follows the scores down as well, once all of a tile's lie more than LOW below it, so that a long row of small weights is
+// not rounded away behind one large one: a tile's weights are kept to 2^-28 of its largest.  m stays within DEEP of the
+// largest score, which keeps the sums below 2^100.
 template <int DT> struct Mma;
 template <> struct Mma<HYENA_DTYPE_BF16> {
-    static constexpr float LAZY = 8.f, SHIFT = 0.f;
+    static constexpr float LAZY = 8.f, SHIFT = 0.f, LOW = 0.f, DEEP = 0.f;
     static __device__ __forceinline__ f32x4 dot(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
     static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf2(lo, hi); }
-    // Weights x, y >= 0 as the exact sum of three terms, none of them 0, so that a weight times an infinite value stays
-    // infinite instead of adding 0 * inf.  A term is the largest bf16 number BELOW what is left (its predecessor cut off),
-    // which leaves 1..2^16 and then 1..2^8 units of the weight's last place.  A weight of 0 counts as the least that
-    // float32 weights go down to.
+    // Weights x, y >= 0 as the exact sum of three terms, none of them 0 unless the weight is, so that a weight times an
+    // infinite value stays infinite instead of adding 0 * inf.  A term is the largest bf16 number BELOW what is left (its
+    // predecessor cut off), which leaves 1..2^16 and then 1..2^8 units of the weight's last place.
     static __device__ __forceinline__ uint32_t below(float x, float y) {
-        return __builtin_amdgcn_perm(__float_as_uint(y) - 1, __float_as_uint(x) - 1, 0x07060302u);
+        return __builtin_amdgcn_perm(__builtin_elementwise_sub_sat(__float_as_uint(y), 1u),
+                                     __builtin_elementwise_sub_sat(__float_as_uint(x), 1u), 0x07060302u);
     }
-    static __device__ __forceinline__ void split(float x, float y, uint32_t (&t)[3]) {
-        x = fmaxf(x, 0x1p-126f), y = fmaxf(y, 0x1p-126f);
+    static __device__ __forceinline__ void split(float x, float y, bool, uint32_t (&t)[3]) {
         t[0] = below(x, y);
         x -= bf_lo(t[0]), y -= bf_hi(t[0]);
         t[1] = below(x, y);
@@ -65,7 +66,7 @@ template <> struct Mma<HYENA_DTYPE_BF16> {
     }
 };
 template <> struct Mma<HYENA_DTYPE_F16> {
-    static constexpr float LAZY = 4.f, SHIFT = 11.f;
+    static constexpr float LAZY = 4.f, SHIFT = 11.f, LOW = 8.f, DEEP = 32.f;
     typedef __attribute__((__vector_size__(2 * sizeof(_Float16)))) _Float16 h2;
     static __device__ __forceinline__ f32x4 dot(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -74,14 +75,19 @@ template <> struct Mma<HYENA_DTYPE_F16> {
         const h2 h = {(_Float16)lo, (_Float16)hi};
         return __builtin_bit_cast(uint32_t, h);
     }
-    // head, rest and rest of the rest, cut off and the last one rounded: all bits of a weight down to 2^-24.  The
-    // smaller two are never 0.
-    static __device__ __forceinline__ void split(float x, float y, uint32_t (&t)[3]) {
+    // Head, rest and rest of the rest, cut off and the last one rounded: all bits of a weight down to 2^-24.  Beside
+    // infinite values (`inf`) the terms of a weight above 0 are 2^-24 at least: a weight times an infinite value stays
+    // infinite instead of adding 0 * inf.
+    typedef __attribute__((__vector_size__(4))) uint16_t u16x2;
+    static __device__ __forceinline__ void split(float x, float y, bool inf, uint32_t (&t)[3]) {
+        const u16x2 least = {(uint16_t)(x > 0.f), (uint16_t)(y > 0.f)};
         const auto a = __builtin_amdgcn_cvt_pkrtz(x, y);
-        x = fmaxf(x - (float)a[0], 0x1p-24f), y = fmaxf(y - (float)a[1], 0x1p-24f);
+        x -= (float)a[0], y -= (float)a[1];
         const auto b = __builtin_amdgcn_cvt_pkrtz(x, y);
         t[0] = __builtin_bit_cast(uint32_t, a), t[1] = __builtin_bit_cast(uint32_t, b);
-        t[2] = pack(fmaxf(x - (float)b[0], 0x1p-24f), fmaxf(y - (float)b[1], 0x1p-24f));
+        t[2] = pack(x - (float)b[0], y - (float)b[1]);
+        if (inf)                                // of numbers >= 0 the larger one has the larger bits
+            for (uint32_t& z : t) z = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, z), least));
     }
     template <bool HI> static __device__ __forceinline__ uint32_t from_f8(uint32_t w) {
         return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, HI));
@@ -196,7 +202,7 @@ struct Walk {
     uint32_t kr[TURN ? 1 : NT][2][NC][KW], vr[NT][8][VB][VW];
     u32x4 kt[TURN ? 2 * NT : 1][TURN ? CPR / 4 : 1], vt[TURNV ? 2 * NT : 1][TURNV ? CPR / 4 : 1];
     f32x4 o[VB * DL];
-    float m, l;
+    float m, mx, l;                         // the weights' reference, the largest score it has followed, their sum
 
     __device__ __forceinline__ Walk(const AttnArgs& args, char* buf) : a(args), lds(buf) {
         lane = lane_id();
@@ -238,8 +244,49 @@ struct Walk {
     __device__ __forceinline__ void nothing() {
 #pragma unroll
         for (int i = 0; i < VB * DL; ++i) o[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
-        m = -INFINITY;
+        m = mx = -INFINITY;
         l = 0.f;
+    }
+
+    // Whether the m of some head has to move for a tile of which `top` is this lane's largest score; and moves it, for
+    // all heads of the tile at once.
+    __device__ __forceinline__ bool off(float top) const {
+        bool move = __any(top > m + M::LAZY);
+        if constexpr (M::LOW > 0) {
+            uint64_t low = __ballot(top < m - M::LOW && m > mx - M::DEEP);      // in all four lanes of a head
+            low &= low >> 32;
+            move |= (low & low >> 16 & 0xffff) != 0;
+        }
+        return move;
+    }
+    __device__ __forceinline__ void follow(float top) {
+        const float t = ceilf(max_over_keys(top));
+        mx = fmaxf(mx, t);
+        const float mn = M::LOW > 0 ? fmaxf(t, mx - M::DEEP) : mx;
+        const float f = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));      // a power of two, without a rounding
+        m = mn;
+        l *= f;
+        const f32x4 g = {__shfl(f, 4 * j), __shfl(f, 4 * j + 1), __shfl(f, 4 * j + 2), __shfl(f, 4 * j + 3)};
+#pragma unroll
+        for (int i = 0; i < VB * DL; ++i) o[i] *= g;
+    }
+
+    // Whether a value of the tile may be infinite (float16; bf16 weights need no care, e4m3 has no infinities).
+    __device__ __forceinline__ bool infinite() const {
+        if constexpr (F8 || DT != HYENA_DTYPE_F16) return false;
+        else {
+            typename M::u16x2 top = {0, 0};
+#pragma unroll
+            for (int g = 0; g < NT; ++g)
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+#pragma unroll
+                    for (int b = 0; b < VB; ++b)
+#pragma unroll
+                        for (int w = 0; w < VW; ++w)
+                            top = __builtin_elementwise_max(top, __builtin_bit_cast(typename M::u16x2, vr[g][i][b][w] & 0x7fff7fffu));
+            return __any(top[0] >= 0x7c00 || top[1] >= 0x7c00);
+        }
     }
 
     // Page of a 16-key piece (wave-uniform), or -1.
@@ -425,14 +472,7 @@ struct Walk {
             for (int i = 0; i < 2 * NT; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) top = fmaxf(top, s[i][e]);
-            if (__any(top > m + M::LAZY)) {                // the maximum moves for all heads of the tile at once
-                const float mn = fmaxf(m, max_over_keys(top)), f = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
-                m = mn;
-                l *= f;
-                const f32x4 g = {__shfl(f, 4 * j), __shfl(f, 4 * j + 1), __shfl(f, 4 * j + 2), __shfl(f, 4 * j + 3)};
-#pragma unroll
-                for (int i = 0; i < VB * DL; ++i) o[i] *= g;
-            }
+            if (off(top)) follow(top);
             const float base = m == -INFINITY ? 0.f : m - M::SHIFT;
 #pragma unroll
             for (int i = 0; i < 2 * NT; ++i)
@@ -441,13 +481,14 @@ struct Walk {
                     s[i][e] = __builtin_amdgcn_exp2f(s[i][e] - base);
                     l += s[i][e];
                 }
+            const bool inf = infinite();
 #pragma unroll
             for (int g = 0; g < NT; ++g) {
                 u32x4 p[3];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     uint32_t t[3];
-                    M::split(s[2 * g + e / 2][2 * (e % 2)], s[2 * g + e / 2][2 * (e % 2) + 1], t);
+                    M::split(s[2 * g + e / 2][2 * (e % 2)], s[2 * g + e / 2][2 * (e % 2) + 1], inf, t);
                     p[0][e] = t[0], p[1][e] = t[1], p[2][e] = t[2];
                 }
 #pragma unroll
