@@ -423,13 +423,15 @@ class RecordedDecodeStep:
         if any(getattr(r, "valid", r.R) < r.R for r in rings if isinstance(r, ops.FirRing)):
             raise NotImplementedError("a cache is still filling up (prompt shorter than a filter): step eagerly")
         mha = ipd["mha"]
-        self.paged = mha.cache if isinstance(mha, PagedAttentionInferenceParams) else None
+        paged = isinstance(mha, PagedAttentionInferenceParams)
+        self.paged = None                       # the cache under record(), from when this object has recorded it
         self.clock = ops.RingClock(rings)
         self.steps = 0
         try:
-            if self.paged is not None:          # pages for every token that fits; the positions move on the device
-                self.room = self.paged.max_len - max(self.paged.lengths())
-                self.paged.record(self.room)
+            if paged:                           # pages for every token that fits; the positions move on the device
+                self.room = mha.cache.max_len - max(mha.cache.lengths())
+                mha.cache.record(self.room)
+                self.paged = mha.cache
             else:
                 mha.offset_dev = torch.tensor([mha.seqlen_offset], dtype=torch.int64, device=dev)
             self.tokens = torch.zeros(batch, 1, dtype=torch.int64, device=dev)
@@ -437,7 +439,7 @@ class RecordedDecodeStep:
             with torch.cuda.graph(self.graph):
                 self.logits = model.forward(self.tokens, ipd)
                 self.clock.advance()
-                if self.paged is None:
+                if not paged:
                     mha.offset_dev.add_(1)
         except BaseException:
             self.release()
@@ -455,5 +457,4 @@ class RecordedDecodeStep:
         self.clock.release()
         if self.paged is not None:
             self.paged.release(self.steps)
-        else:
-            self.ipd["mha"].offset_dev = None
+        self.ipd["mha"].offset_dev = None
