@@ -38,3 +38,45 @@ def test_a_refused_recording_leaves_the_callers_alone():
     cache.release(0)
     advance(ipd, L)
     near(m(ids[:, L + 4:L + 5], ipd)[:, -1], want[:, 5])
+
+
+def test_released_once_and_for_all():
+    m, L, n = model(), 200, 12
+    ids, ipd, want = started(m, L, n, eager=4)
+    rec = RecordedDecodeStep(m, ipd, 2)
+    for i in (5, 6, 7):
+        advance(ipd, L)
+        near(rec(ids[:, L + i - 1:L + i])[:, -1], want[:, i])
+    rec.release()
+    again = RecordedDecodeStep(m, ipd, 2)
+    rec.release()                               # a second time, while another one is in use
+    with pytest.raises(RuntimeError, match="released"):
+        rec(ids[:, :1])
+    assert ipd["mha"].cache.recorded
+    advance(ipd, L)
+    near(again(ids[:, L + 7:L + 8])[:, -1], want[:, 8])
+    again.release()
+    again.release()
+    cache = ipd["mha"].cache
+    assert cache.lengths() == [L + 8] * 2 == cache.lens.tolist()
+    for i in range(9, n):
+        advance(ipd, L)
+        near(m(ids[:, L + i - 1:L + i], ipd)[:, -1], want[:, i])
+    assert cache.lengths() == cache.lens.tolist()
+
+
+def test_a_released_step_on_a_dense_cache_is_refused():
+    m, L = model(), 200
+    ids = tokens(2, L + 8, 4)
+    ipd = m.initialize_inference_params(L + 8)
+    m(ids[:, :L], ipd)
+    for i in range(1, 5):
+        advance(ipd, L)
+        m(ids[:, L + i - 1:L + i], ipd)
+    advance(ipd, L)
+    rec = RecordedDecodeStep(m, ipd, 2)
+    rec(ids[:, L + 4:L + 5])
+    rec.release()
+    rec.release()
+    with pytest.raises(RuntimeError, match="released"):
+        rec(ids[:, :1])

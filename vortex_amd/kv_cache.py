@@ -281,6 +281,7 @@ class PagedKVCache:
         self._refs = [0] * num_pages
         self._pages, self._len = [], []         # per row: its pages in order, the positions it holds
         self.recorded = False                   # a recorded token step uses table and lens: they stay where they are
+        self._room = 0                          # tokens that it was recorded for
         self._set_rows()
 
     @property
@@ -467,7 +468,7 @@ class PagedKVCache:
         """For a recorded token step (a HIP graph): hands out the pages of `tokens` more positions of every row and
         leaves table and lens in place until release().  The step itself calls step()."""
         self.reserve(tokens)
-        self.recorded = True
+        self.recorded, self._room = True, tokens
 
     def step(self):
         """extend(1) on the device alone, inside a recorded step: the host learns of it at release()."""
@@ -476,6 +477,10 @@ class PagedKVCache:
 
     def release(self, steps):
         """Ends record(): `steps` recorded steps have run."""
+        if not self.recorded:
+            raise RuntimeError("no recorded token step to release: its steps are counted already")
+        if not 0 <= steps <= self._room:
+            raise ValueError(f"{steps} steps of a recording for {self._room} tokens")
         self.recorded = False
         self._len = [n + steps for n in self._len]
 

@@ -400,7 +400,7 @@ class RecordedDecodeStep:
     kernels, advanced by one launch at the end of the step) and the attention position (an int64 tensor the
     recorded step increments).  Needs caches that are full (prompt at least as long as the longest FIR filter)
     and one eager token step beforehand, which binds the decode kernels to the caches.  release() hands the
-    positions back to the host-side fields so that eager steps can follow."""
+    positions back to the host-side fields so that eager steps can follow; the object is spent then."""
 
     def __init__(self, model, ipd, batch):
         self.model, self.ipd = model, ipd
@@ -426,7 +426,7 @@ class RecordedDecodeStep:
         paged = isinstance(mha, PagedAttentionInferenceParams)
         self.paged = None                       # the cache under record(), from when this object has recorded it
         self.clock = ops.RingClock(rings)
-        self.steps = 0
+        self.steps, self.released = 0, False
         try:
             if paged:                           # pages for every token that fits; the positions move on the device
                 self.room = mha.cache.max_len - max(mha.cache.lengths())
@@ -446,6 +446,8 @@ class RecordedDecodeStep:
             raise
 
     def __call__(self, tokens):
+        if self.released:
+            raise RuntimeError("this recorded token step was released: record another one")
         if self.paged is not None and self.steps >= self.room:
             raise RuntimeError(f"the paged cache has room for {self.room} recorded tokens")
         self.tokens.copy_(tokens)
@@ -454,6 +456,9 @@ class RecordedDecodeStep:
         return self.logits.clone()                  # the recorded step writes the same buffer every time
 
     def release(self):
+        if self.released:
+            return
+        self.released = True
         self.clock.release()
         if self.paged is not None:
             self.paged.release(self.steps)
