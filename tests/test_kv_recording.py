@@ -1,7 +1,7 @@
 """record / release of a paged cache on the CPU (the device's part is PagedKVCache.step, which a recorded step calls)."""
 import pytest
-import torch
 
+from test_kv_cache import on_cpu                # noqa: F401
 from vortex_amd.kv_cache import PagedKVCache
 
 
@@ -36,3 +36,40 @@ def test_release_refuses_steps_that_cannot_have_run():
         cache.step()
     cache.release(5)
     assert cache.lengths() == [15, 8] == cache.lens.tolist()
+
+
+def test_pages_that_no_step_reached_are_free_again(on_cpu):             # noqa: F811
+    cache = recorded(tokens=54, pages=8)                # to the end of both rows: all eight pages
+    table, lens = cache.table, cache.lens
+    assert cache.free_pages == 0
+    for _ in range(7):
+        cache.step()
+    cache.release(7)                                    # 17 and 10 positions: two pages and one
+    assert cache.free_pages == 5 and cache.table is table and cache.lens is lens
+    assert (cache.table >= 0).sum(1).tolist() == [2, 1] and cache.lens.tolist() == [17, 10]
+    cache.add(1)
+    assert cache.extend([0, 0, 50]).tolist()[-50:] == list(range(50))       # four of the five
+    assert cache.compact() == 7
+    cache.select([0, 1])
+    assert cache.free_pages == 5
+    cache.record(1)                                     # recorded again, and released before any step
+    cache.release(0)
+    assert cache.free_pages == 5 and cache.lengths() == [17, 10] == cache.lens.tolist()
+
+
+def test_pages_reserved_ahead_of_a_recording_stay(on_cpu):              # noqa: F811
+    cache = recorded(tokens=0, pages=8)
+    cache.release(0)
+    cache.reserve([40, 5])                              # 50 positions: four pages; 8: one
+    assert cache.free_pages == 3
+    cache.record(20)
+    assert cache.free_pages == 2
+    cache.release(0)
+    assert cache.free_pages == 3
+    # a fork's recording copies the page that both hold; the copy stays with its row
+    cache.select([1, 1])
+    cache.record(1)
+    pages = [list(p) for p in cache._pages]
+    cache.step()
+    cache.release(1)
+    assert cache._pages == pages and pages[0] != pages[1] and cache.lengths() == [4, 4] and cache.free_pages == 6

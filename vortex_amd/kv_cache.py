@@ -281,7 +281,7 @@ class PagedKVCache:
         self._refs = [0] * num_pages
         self._pages, self._len = [], []         # per row: its pages in order, the positions it holds
         self.recorded = False                   # a recorded token step uses table and lens: they stay where they are
-        self._room = 0                          # tokens that it was recorded for
+        self._room, self._ahead = 0, []         # tokens that it was recorded for, pages that the rows had before
         self._set_rows()
 
     @property
@@ -467,8 +467,9 @@ class PagedKVCache:
     def record(self, tokens):
         """For a recorded token step (a HIP graph): hands out the pages of `tokens` more positions of every row and
         leaves table and lens in place until release().  The step itself calls step()."""
+        ahead = [len(pages) for pages in self._pages]
         self.reserve(tokens)
-        self.recorded, self._room = True, tokens
+        self.recorded, self._room, self._ahead = True, tokens, ahead
 
     def step(self):
         """extend(1) on the device alone, inside a recorded step: the host learns of it at release()."""
@@ -476,13 +477,22 @@ class PagedKVCache:
         return self.lens - 1
 
     def release(self, steps):
-        """Ends record(): `steps` recorded steps have run."""
+        """Ends record(): `steps` recorded steps have run.  Pages that record() handed out and no step has reached are free
+        again."""
         if not self.recorded:
             raise RuntimeError("no recorded token step to release: its steps are counted already")
         if not 0 <= steps <= self._room:
             raise ValueError(f"{steps} steps of a recording for {self._room} tokens")
         self.recorded = False
         self._len = [n + steps for n in self._len]
+        spare = False
+        for pages, n, ahead in zip(self._pages, self._len, self._ahead):
+            keep = max(-(-n // self.page_size), ahead)
+            spare |= keep < len(pages)
+            self._drop(pages[keep:])
+            del pages[keep:]
+        if spare:
+            self._fill()
 
     def compact(self):
         """Moves the pages in use to the lowest ids (one launch over all layers) and returns how many they are."""
