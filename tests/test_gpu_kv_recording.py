@@ -80,3 +80,50 @@ def test_a_released_step_on_a_dense_cache_is_refused():
     rec.release()
     with pytest.raises(RuntimeError, match="released"):
         rec(ids[:, :1])
+
+
+def test_recording_on_a_pool_smaller_than_every_rows_longest():
+    # 2 rows of up to 800 tokens would need 100 pages; 2 * 14 are there
+    m, L, n = model(), 200, 16
+    ids, ipd, want = started(m, L, n, eager=4, max_seqlen=800, num_pages=2 * 14)
+    cache = ipd["mha"].cache
+    with pytest.raises(RuntimeError, match="pages needed"):
+        RecordedDecodeStep(m, ipd, 2)
+    for tokens in (0, -3):
+        with pytest.raises(ValueError):
+            RecordedDecodeStep(m, ipd, 2, tokens=tokens)
+    with pytest.raises(ValueError, match="more positions"):
+        RecordedDecodeStep(m, ipd, 2, tokens=700)
+    assert not cache.recorded and cache.lengths() == [L + 4] * 2 and cache.free_pages == 2
+    rec = RecordedDecodeStep(m, ipd, 2, tokens=6)
+    assert cache.free_pages == 0                        # a page each from position 208 on
+    for i in range(5, 11):
+        advance(ipd, L)
+        near(rec(ids[:, L + i - 1:L + i])[:, -1], want[:, i])
+    with pytest.raises(RuntimeError, match="6 tokens"):
+        rec(ids[:, :1])
+    rec.release()
+    assert cache.free_pages == 0 and cache.lengths() == [L + 10] * 2 == cache.lens.tolist()
+    advance(ipd, L)
+    near(m(ids[:, L + 10:L + 11], ipd)[:, -1], want[:, 11])
+    rec = RecordedDecodeStep(m, ipd, 2, tokens=4)       # and again
+    for i in range(12, n):
+        advance(ipd, L)
+        near(rec(ids[:, L + i - 1:L + i])[:, -1], want[:, i])
+    rec.release()
+    assert cache.lengths() == [L + 15] * 2 == cache.lens.tolist()
+
+
+def test_a_recording_for_some_tokens_on_a_dense_cache():
+    m, L = model(), 200
+    ids = tokens(2, L + 8, 4)
+    ipd = m.initialize_inference_params(L + 8)
+    m(ids[:, :L], ipd)
+    for i in range(1, 5):
+        advance(ipd, L)
+        m(ids[:, L + i - 1:L + i], ipd)
+    advance(ipd, L)
+    rec = RecordedDecodeStep(m, ipd, 2, tokens=1)
+    rec(ids[:, L + 4:L + 5])
+    with pytest.raises(RuntimeError, match="1 token"):
+        rec(ids[:, L + 5:L + 6])

@@ -400,9 +400,13 @@ class RecordedDecodeStep:
     kernels, advanced by one launch at the end of the step) and the attention position (an int64 tensor the
     recorded step increments).  Needs caches that are full (prompt at least as long as the longest FIR filter)
     and one eager token step beforehand, which binds the decode kernels to the caches.  release() hands the
-    positions back to the host-side fields so that eager steps can follow; the object is spent then."""
+    positions back to the host-side fields so that eager steps can follow; the object is spent then.
 
-    def __init__(self, model, ipd, batch):
+    tokens: how many will be stepped at most.  A paged cache hands out their pages ahead (release() takes back the ones not
+    reached); without it, those of every token up to max_seqlen, which a cache of fewer pages than rows * max_seqlen
+    refuses."""
+
+    def __init__(self, model, ipd, batch, tokens=None):
         self.model, self.ipd = model, ipd
         dev = model.embedding.weight.device
         rings = []
@@ -427,9 +431,13 @@ class RecordedDecodeStep:
         self.paged = None                       # the cache under record(), from when this object has recorded it
         self.clock = ops.RingClock(rings)
         self.steps, self.released = 0, False
+        self.room = tokens
         try:
-            if paged:                           # pages for every token that fits; the positions move on the device
-                self.room = mha.cache.max_len - max(mha.cache.lengths())
+            if tokens is not None and tokens < 1:
+                raise ValueError(f"a recording for {tokens} tokens")
+            if paged:                           # the positions move on the device
+                if tokens is None:
+                    self.room = mha.cache.max_len - max(mha.cache.lengths())
                 mha.cache.record(self.room)
                 self.paged = mha.cache
             else:
@@ -448,8 +456,8 @@ class RecordedDecodeStep:
     def __call__(self, tokens):
         if self.released:
             raise RuntimeError("this recorded token step was released: record another one")
-        if self.paged is not None and self.steps >= self.room:
-            raise RuntimeError(f"the paged cache has room for {self.room} recorded tokens")
+        if self.room is not None and self.steps >= self.room:
+            raise RuntimeError(f"recorded for {self.room} tokens, which have been stepped")
         self.tokens.copy_(tokens)
         self.graph.replay()
         self.steps += 1
