@@ -461,7 +461,8 @@ int hyena_fir_layer_fwd(const hyena_proj_fwd* proj,
  * Rules (others: HYENA_ENOSUP / HYENA_EALIGN): head_dim a multiple of 8 up to 256; page_size a power of two from 16 to
  * 65536; a table row names at most 2^30 positions; strides multiples of 8 elements (that of a dimension of one element
  * is not looked at), pointers 16-byte aligned; in attention the positions of a page lie at most 2^27 bytes apart; an
- * append takes at most 32768 heads, whose rows for 16 tokens lie within 2^32 bytes. */
+ * append takes at most 32768 heads, whose rows for 16 tokens lie within 2^32 bytes.  What does not fit one launch is
+ * HYENA_EINVAL: 2^26 (sequence, head) pairs in attention, 2^24 to 2^28 tokens in an append (by the size of a token). */
 typedef struct hyena_kv_side {
     void* ptr;
     int64_t page_stride, head_stride, slot_stride;

@@ -821,10 +821,12 @@ extern "C" int hyena_attn_step(const hyena_kv_pages* kv, const hyena_heads* q, c
     // a lane's place in a 16-key piece is a 32-bit offset
     if (a.kv.k.slot_stride < 0 || a.kv.v.slot_stride < 0 || a.kv.k.slot_stride > (1 << 27) || a.kv.v.slot_stride > (1 << 27))
         return hyena_fail(HYENA_ENOSUP, "%s: positions of a page that lie %lld bytes apart", who, (long long)a.kv.k.slot_stride);
-    if (kv->sequences * heads >= (1LL << 31))
-        return hyena_fail(HYENA_EINVAL, "%s: %lld sequences of %lld heads", who, (long long)kv->sequences, (long long)heads);
     const int64_t need = hyena_attn_step_ws_bytes(kv, heads);
     const bool few = short_rows(kv, heads);
+    // a block of up to 512 threads per (sequence, key head, query tile), or 64 threads per (sequence, head)
+    if (kv->sequences * heads > KV_GRID_THREADS / (few ? 512 : 64) - 4)
+        return hyena_fail(HYENA_EINVAL, "%s: %lld sequences of %lld heads are too many for one call", who,
+                          (long long)kv->sequences, (long long)heads);
     if (!few && (!ws || ws_bytes < need || ((uintptr_t)ws & 15)))
         return hyena_fail(HYENA_EINVAL, "%s: workspace of %lld bytes (16-byte aligned), %lld needed", who, (long long)ws_bytes,
                           (long long)need);

@@ -49,6 +49,8 @@ struct KvHeads {
     int64_t token_stride, head_stride;                  // bytes
 };
 
+constexpr int64_t KV_GRID_THREADS = (1LL << 32) - 1;   // of a launch in one dimension
+
 static inline int64_t kv_elem_bytes(int dtype) { return dtype == HYENA_DTYPE_F8E4M3 ? 1 : 2; }
 
 // Checks a cache description and fills its device copy; 0 or a HYENA_E* code.

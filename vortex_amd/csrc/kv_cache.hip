@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(256) copy_pages_kernel(const char* src_base, i
 }
 
 template <int DT, bool F8, int VEC, bool IL, bool STREAM>
-void launch_append(AppendArgs& a, hipStream_t s) {
+int launch_append(AppendArgs& a, hipStream_t s, const char* who) {
     // A block's rounds: up to 2 * BATCH over as many tokens as leave the fewest threads of a round idle, if that makes
     // enough blocks for every compute unit to hold a few (1024); else fewer, down to one round of one token a block
     // (the angles of a token are then made in several blocks, which costs less than waiting for one).
@@ -293,29 +293,31 @@ void launch_append(AppendArgs& a, hipStream_t s) {
         if (rounds(n) * bt <= rounds(bt) * n) bt = n;
     int64_t per = rounds(bt);
     const int64_t blocks = (a.tokens + bt - 1) / bt;
+    if (blocks > KV_GRID_THREADS / APPEND_THREADS)
+        return hyena_fail(HYENA_EINVAL, "%s: %lld tokens are too many for one call", who, (long long)a.tokens);
     const int64_t split = std::min<int64_t>(per, std::max<int64_t>((per + 2 * BATCH - 1) / (2 * BATCH), 1024 / blocks));
     per = (per + split - 1) / split;
     a.block_tokens = (int32_t)bt;
     a.block_rounds = (int32_t)per;
     hipLaunchKernelGGL((rotary_append_kernel<DT, F8, VEC, IL, STREAM>), dim3((unsigned)blocks, (unsigned)((rounds(bt) + per - 1) / per)),
                        dim3(APPEND_THREADS), 0, s, a);
+    return hyena_check_launch(who);
 }
 
 template <int DT, bool F8>
-void launch_append_type(AppendArgs& a, bool il, hipStream_t s) {
+int launch_append_type(AppendArgs& a, bool il, hipStream_t s, const char* who) {
     // Pieces of 8 elements where the rotary part allows them, of 2 or 1 where it ends elsewhere.  Non-temporal accesses
     // where the rows of q and k, read and written, are more than half of the last-level cache (8192 tokens of 96 rows of 128: 96.6
     // against 86.7 us); below, the rows stay there for the attention that follows (460 K rows of 64: 15.7 against 17.1).
     const int half = a.half;
     const bool stream = a.tokens * (a.role[0].heads + a.role[1].heads) * a.kv.head_dim * 4 > (128 << 20);
     if (il) {
-        if (half % 4 == 0) stream ? launch_append<DT, F8, 8, true, true>(a, s) : launch_append<DT, F8, 8, true, false>(a, s);
-        else launch_append<DT, F8, 2, true, false>(a, s);
-    } else {
-        if (half % 8 == 0) stream ? launch_append<DT, F8, 8, false, true>(a, s) : launch_append<DT, F8, 8, false, false>(a, s);
-        else if (half % 2 == 0) launch_append<DT, F8, 2, false, false>(a, s);
-        else launch_append<DT, F8, 1, false, false>(a, s);
+        if (half % 4 == 0) return stream ? launch_append<DT, F8, 8, true, true>(a, s, who) : launch_append<DT, F8, 8, true, false>(a, s, who);
+        return launch_append<DT, F8, 2, true, false>(a, s, who);
     }
+    if (half % 8 == 0) return stream ? launch_append<DT, F8, 8, false, true>(a, s, who) : launch_append<DT, F8, 8, false, false>(a, s, who);
+    if (half % 2 == 0) return launch_append<DT, F8, 2, false, false>(a, s, who);
+    return launch_append<DT, F8, 1, false, false>(a, s, who);
 }
 
 }  // namespace
@@ -369,9 +371,9 @@ extern "C" int hyena_rotary_append(const hyena_kv_pages* kv, const hyena_heads* 
     a.tokens = tokens;
     hipStream_t s = (hipStream_t)stream;
     const bool f8 = kv->dtype == HYENA_DTYPE_F8E4M3, il = interleaved != 0;
-    if (dtype == HYENA_DTYPE_BF16) f8 ? launch_append_type<HYENA_DTYPE_BF16, true>(a, il, s) : launch_append_type<HYENA_DTYPE_BF16, false>(a, il, s);
-    else f8 ? launch_append_type<HYENA_DTYPE_F16, true>(a, il, s) : launch_append_type<HYENA_DTYPE_F16, false>(a, il, s);
-    return hyena_check_launch(who);
+    if (dtype == HYENA_DTYPE_BF16)
+        return f8 ? launch_append_type<HYENA_DTYPE_BF16, true>(a, il, s, who) : launch_append_type<HYENA_DTYPE_BF16, false>(a, il, s, who);
+    return f8 ? launch_append_type<HYENA_DTYPE_F16, true>(a, il, s, who) : launch_append_type<HYENA_DTYPE_F16, false>(a, il, s, who);
 }
 
 extern "C" int hyena_kv_copy_pages(const hyena_kv_pools* src_pools, const hyena_kv_pools* dst_pools, int64_t pools,
@@ -392,12 +394,18 @@ extern "C" int hyena_kv_copy_pages(const hyena_kv_pools* src_pools, const hyena_
     const int wide = (at & 15) == 0;
     const bool much = copies * pools > (64 << 20) / page_bytes;
     const int64_t piece = much ? 4096 : 16384, pieces = (page_bytes + piece - 1) / piece;
-    if (copies * pieces >= (1LL << 31))
+    constexpr int64_t MOST = KV_GRID_THREADS / 256;     // blocks of a launch; more pairs take several
+    if (copies * pieces >= (1LL << 31) || pieces > MOST)
         return hyena_fail(HYENA_EINVAL, "%s: %lld copies of %lld bytes are too many for one call", who, (long long)copies,
                           (long long)page_bytes);
-    hipLaunchKernelGGL(much ? copy_pages_kernel<1> : copy_pages_kernel<4>, dim3((unsigned)(copies * pieces), (unsigned)pools),
-                       dim3(256), 0, (hipStream_t)stream, (const char*)src_pools->base, src_pools->pool_stride,
-                       src_pools->page_stride, src_pools->pages, (char*)dst_pools->base, dst_pools->pool_stride,
-                       dst_pools->page_stride, dst_pools->pages, page_bytes, (int32_t)pieces, src, dst, wide);
-    return hyena_check_launch(who);
+    for (int64_t done = 0; done < copies;) {
+        const int64_t n = std::min(copies - done, MOST / pieces);
+        hipLaunchKernelGGL(much ? copy_pages_kernel<1> : copy_pages_kernel<4>, dim3((unsigned)(n * pieces), (unsigned)pools),
+                           dim3(256), 0, (hipStream_t)stream, (const char*)src_pools->base, src_pools->pool_stride,
+                           src_pools->page_stride, src_pools->pages, (char*)dst_pools->base, dst_pools->pool_stride,
+                           dst_pools->page_stride, dst_pools->pages, page_bytes, (int32_t)pieces, src + done, dst + done, wide);
+        if (const int rc = hyena_check_launch(who)) return rc;
+        done += n;
+    }
+    return 0;
 }
