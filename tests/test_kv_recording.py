@@ -73,3 +73,15 @@ def test_pages_reserved_ahead_of_a_recording_stay(on_cpu):              # noqa: 
     cache.step()
     cache.release(1)
     assert cache._pages == pages and pages[0] != pages[1] and cache.lengths() == [4, 4] and cache.free_pages == 6
+
+
+def test_what_the_host_cannot_know_is_refused(on_cpu):                  # noqa: F811
+    cache = recorded(tokens=5)
+    cache.step()
+    with pytest.raises(RuntimeError, match="recorded"):
+        cache.dense(0)                                  # by the host's lengths it would leave the last position out
+    cache.release(1)
+    assert cache.dense(0)[0].shape == (2, 1, 11, 8)
+    with pytest.raises(RuntimeError, match="record"):
+        cache.step()                                    # nothing would tell the host
+    assert cache.lens.tolist() == cache.lengths() == [11, 4]

@@ -310,6 +310,7 @@ class PagedKVCache:
         """Keys and values of layer i as two [rows, kv_heads, max(lengths), head_dim] tensors of the activations' type,
         zero behind a row's end: for attention of many new tokens at once, where reading the pages once into rows is
         cheaper than reading them for every token."""
+        self._not_recorded()                    # the host does not know how far a recorded step has gone
         n = max(self._len, default=0)
         w = -(-n // self.page_size)
         at = self.table[:, :w].clamp(min=0).long()
@@ -473,6 +474,8 @@ class PagedKVCache:
 
     def step(self):
         """extend(1) on the device alone, inside a recorded step: the host learns of it at release()."""
+        if not self.recorded:
+            raise RuntimeError("step() moves the lengths of a cache under record(): extend(1) counts a token on the host too")
         self.lens.add_(1)
         return self.lens - 1
 
