@@ -127,3 +127,20 @@ def test_a_recording_for_some_tokens_on_a_dense_cache():
     rec(ids[:, L + 4:L + 5])
     with pytest.raises(RuntimeError, match="1 token"):
         rec(ids[:, L + 5:L + 6])
+
+
+def test_an_eager_token_between_replays_is_refused():
+    # it would move the lengths on the device without anybody counting it
+    m, L, n = model(pattern=("hcs", "attn"), num_layers=2), 200, 9
+    ids, ipd, want = started(m, L, n, eager=4)
+    rec = RecordedDecodeStep(m, ipd, 2)
+    for i in (5, 6):
+        advance(ipd, L)
+        near(rec(ids[:, L + i - 1:L + i])[:, -1], want[:, i])
+        with pytest.raises(RuntimeError, match="release"):
+            m(ids[:, L + i - 1:L + i], ipd)
+    rec.release()
+    cache = ipd["mha"].cache
+    assert cache.lengths() == [L + 6] * 2 == cache.lens.tolist()
+    advance(ipd, L)
+    near(m(ids[:, L + 6:L + 7], ipd)[:, -1], want[:, 7])

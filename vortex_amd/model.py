@@ -103,11 +103,14 @@ class PagedAttentionInferenceParams:
         self.seqlen_offset = 0      # kept by callers as for the other caches; the cache counts for itself
         self.offset_dev = None
         self.positions, self.first = None, False
+        self.replayed = False       # a RecordedDecodeStep counts this cache's tokens
 
     def begin(self, batch, length):
         """Makes room for a step's tokens; the model calls it ahead of the blocks."""
         if batch != self.cache.rows:
             raise ValueError(f"a batch of {batch} on a cache of {self.cache.rows} sequences")
+        if self.replayed:
+            raise RuntimeError("a recorded token step counts these caches' tokens: release it first")
         if self.cache.recorded:
             if length != 1:
                 raise RuntimeError("a recorded token step takes one token")
@@ -449,6 +452,8 @@ class RecordedDecodeStep:
                 self.clock.advance()
                 if not paged:
                     mha.offset_dev.add_(1)
+            if paged:
+                mha.replayed = True
         except BaseException:
             self.release()
             raise
@@ -470,4 +475,5 @@ class RecordedDecodeStep:
         self.clock.release()
         if self.paged is not None:
             self.paged.release(self.steps)
+            self.ipd["mha"].replayed = False
         self.ipd["mha"].offset_dev = None
