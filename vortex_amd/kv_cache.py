@@ -77,7 +77,7 @@ def _scale(t, heads, name):
 def _kv(k_pages, v_pages, table, k_scale, v_scale, act):
     """hyena_kv_pages of one layer's cache for activations of type `act`, and (kv_heads, head_dim, sequences)."""
     shape = k_pages.shape
-    if len(shape) != 4 or shape != v_pages.shape:
+    if len(shape) != 4 or shape != v_pages.shape or not shape[1]:
         raise ValueError("k_pages and v_pages must be [pages, kv_heads, page_size, head_dim] tensors of one shape, got "
                          f"{tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
     dtype = k_pages.dtype
