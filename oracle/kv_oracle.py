@@ -24,7 +24,8 @@ def attn(q, k_pages, v_pages, table, lens, scale, k_scale=None, v_scale=None):
         the product (3 * 2^-24 |s|), so a weight is off by a relative d = max_j of that, plus 2^-21 for the power of two
         and its argument's subtraction (|s - max| 2^-24 below 2^-17 where the weight is not negligible, counted there);
         numerator and denominator both carry it: 2 d A
-      weights kept as two 16-bit terms: 2^-16 A (bf16); in float16 terms also 2^-25 per weight of the absolute kind
+      weights kept as three 16-bit terms: exactly in bf16; in float16 to multiples of 2^-24 where the largest weight is
+        2^10 at least, so 2^-35 of it for every value, whatever its weight
       sums over n positions and the join of parts: (n + 64) 2^-24 A, twice (numerator, denominator)"""
     q, table, lens = q.detach().cpu(), table.cpu(), lens.cpu()
     kp, vp = k_pages.detach().cpu(), v_pages.detach().cpu()
@@ -53,8 +54,9 @@ def attn(q, k_pages, v_pages, table, lens, scale, k_scale=None, v_scale=None):
             A = w @ val.abs() / den
             d = (hd * 2.0 ** -24 * (x.abs() @ key.abs().T) * abs(scale)).amax(-1, keepdim=True) \
                 + 3 * 2.0 ** -24 * s.abs().amax(-1, keepdim=True) + 2.0 ** -17
-            slack[b, h * g:(h + 1) * g] = A * (2 * d + 2.0 ** -16 + (2 * len(spots) + 128) * 2.0 ** -24) \
-                + 2.0 ** -25 * val.abs().sum(0) / den
+            slack[b, h * g:(h + 1) * g] = A * (2 * d + (2 * len(spots) + 128) * 2.0 ** -24)
+            if q.dtype == torch.float16:
+                slack[b, h * g:(h + 1) * g] += 2.0 ** -35 * val.abs().sum(0) / den
     return out, slack
 
 
