@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+import kv_markers as M
 from oracle import kv_oracle as K
 
 
@@ -20,3 +21,18 @@ def test_large_values_behind_vanishing_weights_get_no_slack(dtype, most):
     assert bool((y == 1.0).all()) and bool((slack < most).all())
     with pytest.raises(AssertionError):
         K.assert_rounds_to((y * (1 + 2.0 ** -6)).to(dtype), y, slack)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("step,lost", [(1, 32), (7, 21)])
+def test_a_lost_or_doubled_tile_of_a_long_row_shows(step, lost, dtype):
+    # the markers of kv_markers.py on 70000 positions: 32 of them lost or doubled, or three of those that count
+    n, hd = 70000, 64
+    y = M.result(n, hd, step)
+    K.assert_rounds_to(K.rounded(y, dtype).to(dtype), y, y * M.SLACK)
+    for at in (0, 34000, n - lost):
+        j = torch.arange(n)
+        for used in (torch.cat([j[:at], j[at + lost:]]), torch.cat([j, j[at:at + lost]])):
+            bad = K.rounded(M.result(n, hd, step, used=used), dtype).to(dtype)
+            with pytest.raises(AssertionError):
+                K.assert_rounds_to(bad, y, y * M.SLACK)
