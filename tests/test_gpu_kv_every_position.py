@@ -27,9 +27,10 @@ def paged(k, v, kv_heads, page, seed, spare=3):
     for x in (k, v):
         full = torch.full((need * page, hd), float("nan"))
         full[:n] = x.float()
-        p = torch.full((need + spare, kv_heads, page, hd), float("nan"))
-        p[ids] = full.view(need, 1, page, hd).expand(-1, kv_heads, -1, -1)
-        out.append(p.to(x.dtype).to(DEV))
+        raw = lambda y: y.to(x.dtype).view(torch.uint8 if x.dtype == FP8 else x.dtype).to(DEV)
+        p = raw(torch.tensor(float("nan"))).expand(need + spare, kv_heads, page, hd).contiguous()
+        p[ids.to(DEV)] = raw(full.view(need, 1, page, hd))
+        out.append(p.view(x.dtype))
     return out[0], out[1], ids.to(torch.int32)
 
 
@@ -60,15 +61,17 @@ def test_every_position_counts_once(override, lens, kv_heads, group, hd, page, d
     K.assert_rounds_to(got, want, want * M.SLACK, f"holes, {lens[:3]} {hd} {step}")
 
 
+@pytest.mark.parametrize("room", [True, False])
 @pytest.mark.parametrize("step", [1, 7])
 @pytest.mark.parametrize("dtype,fp8", [(BF, False), (F16, False), (BF, True), (F16, True)])
 @pytest.mark.parametrize("hd", [32, 64, 80, 128, 160, 256])
-def test_reads_beyond_the_last_level_cache(hd, dtype, fp8, step):
-    # more than 128 MiB of reads in a call: its loads are non-temporal.  The sequences are one, read to different lengths
+def test_reads_beyond_the_last_level_cache(hd, dtype, fp8, step, room):
+    # more than 128 MiB of reads in a call: its loads are non-temporal where the pages could all be different ones (room).
+    # The sequences are one, read to different lengths
     kv_heads, group, page, longest, t = 2, 3, 64, 5001, FP8 if fp8 else dtype
-    k, v, ids = paged(*M.rows(longest, hd, step, t, hd), kv_heads, page, hd)
-    B = (160 << 20) // (longest * kv_heads * hd * 2 * k.element_size()) + 1
+    B = (160 << 20) // (longest * kv_heads * hd * 2 * t.itemsize) + 1
     lens = [longest - 7 * b % 600 for b in range(B)]
+    k, v, ids = paged(*M.rows(longest, hd, step, t, hd), kv_heads, page, hd, spare=sum(lens) // page + B if room else 3)
     assert sum(lens) * kv_heads * hd * 2 * k.element_size() > 130 << 20
     want = torch.stack([M.result(n, hd, step, of=longest) for n in lens])[:, None].expand(-1, kv_heads * group, -1)
     got = attn_step(query(B, kv_heads * group, hd, dtype), k, v, ids[None].expand(B, -1).to(DEV),
@@ -76,17 +79,19 @@ def test_reads_beyond_the_last_level_cache(hd, dtype, fp8, step):
     K.assert_rounds_to(got, want, want * M.SLACK, f"{B} x {longest}, {hd}")
 
 
+@pytest.mark.parametrize("room", [True, False])
 @pytest.mark.parametrize("dtype,fp8,hd,group", [(BF, False, 128, 1), (F16, False, 64, 8), (BF, True, 128, 8), (BF, False, 80, 4)])
-def test_random_values_beyond_the_last_level_cache(dtype, fp8, hd, group):
+def test_random_values_beyond_the_last_level_cache(dtype, fp8, hd, group, room):
     # four different queries, each in many rows of the call
     n, kv_heads, page, t = 3001, 2, 64, FP8 if fp8 else dtype
     g = torch.Generator().manual_seed(hd)
     scale = 30.0 if fp8 else 1.0
-    k, v, ids = paged((scale * torch.randn(n, hd, generator=g)).to(t), (scale * torch.randn(n, hd, generator=g)).to(t), kv_heads, page, 5)
+    R = (140 << 20) // (2048 * kv_heads * hd * 2 * t.itemsize * 4) + 1
+    k, v, ids = paged((scale * torch.randn(n, hd, generator=g)).to(t), (scale * torch.randn(n, hd, generator=g)).to(t), kv_heads, page,
+                      5, spare=4 * R * (n // page + 1) if room else 3)
     ks = vs = torch.tensor([0.02, 0.05], device=DEV) if fp8 else None
     lens = torch.tensor([n, n - 1, 2048, 2500], dtype=torch.int32)
     q = (2 * torch.randn(4, kv_heads * group, hd, generator=g)).to(dtype)
     y, slack = K.attn(q, k, v, ids[None].expand(4, -1), lens, hd ** -0.5, ks, vs)
-    R = (140 << 20) // (2048 * kv_heads * hd * 2 * k.element_size() * 4) + 1
     got = attn_step(q.repeat(R, 1, 1).to(DEV), k, v, ids[None].expand(4 * R, -1).to(DEV), lens.repeat(R).to(DEV), k_scale=ks, v_scale=vs)
     K.assert_rounds_to(got, y.repeat(R, 1, 1), slack.repeat(R, 1, 1))
