@@ -568,8 +568,8 @@ struct Walk {
 // on the device, and this is even for any of them.  A row inside one run is finished here; the first and the last row
 // of a run may be parts (slots 2w and 2w + 1), which attn_join_kernel adds up.
 // Measured, both launches: one sequence of 131072 keys, 32 heads of 128, bf16: 328 us, 6.5 TB/s of reads (7.0 is what
-// reads alone reach); 64 sequences of 0..4096 keys: 366 us, 6.4 TB/s; 32 of up to 32768, 8 key heads, e4m3: 189 us,
-// 6.0 TB/s; one of 2000 keys (33 MB): 14 us, of which 8 are two launches without work.
+// reads alone reach); 64 sequences of 0..4096 keys: 367 us, 6.4 TB/s; 32 of up to 32768, 8 key heads, e4m3: 190 us,
+// 6.0 TB/s; one of 2000 keys (33 MB): 14.8 us, of which 8 are two launches without work.
 template <int DT, bool F8, int HDP, bool PAD>
 __global__ void __launch_bounds__(64 * WAVES, HDP > 128 ? 1 : 2) attn_walk_kernel(AttnArgs a) {
     typedef Walk<DT, F8, HDP, PAD> W;
@@ -622,7 +622,8 @@ __global__ void __launch_bounds__(64 * WAVES, HDP > 128 ? 1 : 2) attn_walk_kerne
 }
 
 // Short rows: one block per row, its wavefronts take the tiles in turn and add up their parts in LDS.  One launch, bound
-// by its chain of latencies (table, keys, values): 203 keys of 32 heads 5.8 us where the even cut takes 8.8.
+// by its chain of latencies (table, keys, values): 203 keys of 32 heads 6.4 us; 256 keys, in a recorded graph, 6.6 us
+// where the even cut takes 9.1.
 template <int HDP> constexpr int short_waves() { return HDP > 128 ? 4 : 8; }
 
 template <int DT, bool F8, int HDP, bool PAD>
@@ -755,8 +756,17 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
 int padded(int64_t hd) { return hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
 
 // Whether every row is short: what the table can name (lengths are on the device) keeps a block's wavefronts at a few
-// tiles each, and the blocks are few enough to run at once or nearly.  Even cut against this form, heads of 128 in bf16:
-// 32 rows of 512 KiB 12.6 / 10.5 us, of 1 MiB 14.1 / 15.9; 512 rows of 512 KiB 52 / 50; 2048 rows of 32 KiB 18.5 / 33.
+// tiles each, and the blocks are few enough to run at once or nearly.  Even cut against this form in us, calls in a recorded
+// graph:                          heads of 128, bf16   64, bf16      64, float16   128, e4m3
+//   32 rows of 128 KiB               9.1 /  6.6         9.6 /  7.5    9.8 /  7.7   10.1 /  7.8
+//   32 rows of 512 KiB              11.8 / 11.3        13.0 / 14.5   12.8 / 14.7   13.6 / 16.9
+//   32 rows of 1 MiB                14.0 / 16.6        14.9 / 22.6   14.8 / 23.3   15.9 / 27.5
+//   128 rows of 512 KiB             19.5 / 14.4        19.2 / 16.0   19.5 / 16.5   20.0 / 18.4
+//   512 rows of 32 KiB              12.5 / 10.6        12.6 / 10.7   12.8 / 11.1   13.2 / 12.1
+//   512 rows of 512 KiB             50.9 / 49.8        49.1 / 53.1   48.8 / 53.8   50.8 / 52.3
+//   1024 rows of 32 KiB             13.4 / 18.7        13.7 / 18.7   13.9 / 19.4   14.8 / 21.8
+//   2048 rows of 32 KiB             18.1 / 32.3        18.9 / 33.7   19.5 / 34.8   20.4 / 40.1
+// The border of 512 KiB is that of heads of 128 in bf16; the others lose up to 4 us at it with few rows or many.
 bool short_rows(const hyena_kv_pages* kv, int64_t heads) {
     const int64_t ov = hyena_override(HYENA_OV_ATTN_SHORT);
     if (ov >= 0) return ov != 0;
@@ -765,9 +775,11 @@ bool short_rows(const hyena_kv_pages* kv, int64_t heads) {
     return bytes <= (512 << 10) && rows <= 512;
 }
 
-// Wavefronts of the even cut.  One per SIMD reads long rows fastest (1.07 GB in 256 rows: e4m3 196 us against 202 with
-// two, bf16 174 against 180) and leaves fewer parts to join; with many rows each wavefront changes rows often, and a
-// second one on the SIMD works meanwhile (2048 rows of up to 4096 keys: 372 us against 397 with one).
+// Wavefronts of the even cut.  One per SIMD leaves fewer parts to join: 2000 keys of 32 heads in bf16 14.3 us against 16.3
+// with two, 8000 keys 31.7 / 31.5, 32768 keys 87 / 92, 8 sequences of 2048 48 / 53, 16 of 4096 and 8191 with 4 key heads of
+// 64 in float16 20.0 / 21.1 and 32.6 / 33.2, 32 of 4096 with 8 key heads in e4m3 54 / 59; equal on long rows (131072 keys
+// 335 / 332).  With many rows each wavefront changes rows often, and a second one on the SIMD works meanwhile (2048 rows of
+// up to 4096 keys: 385 us against 390 with one).
 int64_t waves_for(const hyena_kv_pages* kv, int64_t heads) {
     const int64_t rows = kv->sequences * kv->kv_heads * ((heads / kv->kv_heads + 15) / 16);
     return kv->head_dim <= 128 && rows > 1024 ? 2048 : 1024;
@@ -782,7 +794,7 @@ void launch(const AttnArgs& a, bool few, hipStream_t s) {
     }
     hipLaunchKernelGGL((attn_walk_kernel<DT, F8, HDP, PAD>), dim3(a.waves / WAVES), dim3(64 * WAVES), 0, s, a);
     // many heads have few parts each: one wavefront a head instead of a block (2048 sequences of 32
-    // keys, 32 heads: 123 -> 79 us with the walk)
+    // keys, 32 heads on 8: 123 us with the walk, 80 with a wavefront: 67 for the walk, 13 for the join)
     const int64_t heads = (int64_t)a.kv.sequences * a.heads;
     if (heads > 1024) hipLaunchKernelGGL((attn_join_kernel<DT, HDP, 64>), dim3((unsigned)((heads + 3) / 4)), dim3(256), 0, s, a);
     else hipLaunchKernelGGL((attn_join_kernel<DT, HDP, 256>), dim3((unsigned)heads), dim3(256), 0, s, a);

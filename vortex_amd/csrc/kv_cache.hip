@@ -125,7 +125,8 @@ template <int DT, int VEC, bool STREAM> struct Piece {
 // neighbouring pieces, then neighbouring heads, so a wavefront moves whole rows.  Rounds go over the (token, head) rows of
 // q, then k, then v: what a round works on is uniform, which keeps its addresses in scalar registers.  The first BATCH
 // rounds are requested before the block makes the cosines and sines of its tokens in LDS (one pair a thread: an angle
-// in float64 costs as much as rotating a dozen heads).
+// in float64 costs as much as rotating a dozen heads).  The angle is rounded to float32 once it is reduced to half a turn:
+// off by at most pi 2^-24, and the result by as much of the pair's length, where the last rounding takes 2^-8 (float16 2^-11).
 // Measured: 8192 tokens, 32 heads of 128 with their keys and values, dense keys too, bf16: 80-85 us, 5.5-5.9 TB/s read and
 // written; one token 4.5 us.
 template <int DT, bool F8, int VEC, bool IL, bool STREAM>

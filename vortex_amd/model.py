@@ -30,8 +30,11 @@ EVO2_7B = dict(
 )
 
 
-# New tokens of a continuation that attn_step takes one by one; more read the pages once into rows (32 heads of 128 behind
-# 8192 positions: 16 tokens 0.20 against 0.68 ms, 64 tokens 1.17 against 0.74).
+# New tokens of a continuation that attn_step takes one by one; more read the pages once into rows.  One by one against
+# gathered, 32 heads of 128, bf16, ms: 32 tokens behind 512 / 2048 / 8192 / 32768 positions 0.04 / 0.09 / 0.30 / 1.1 against
+# 0.14 / 0.23 / 0.70 / 2.9, 64 tokens 0.07 / 0.32 / 1.24 / 4.4 against 0.14 / 0.25 / 0.74 / 3.1; four sequences behind 8192,
+# 32 tokens 0.82 against 1.55, 64 tokens 4.2 against 1.6.  Pages in 8 bits favour single queries further on (64 tokens behind
+# 8192 0.38 against 1.02, 128 tokens 1.19 against 1.02).
 PAGED_QUERIES = 32
 SEQ_MAJOR = "auto"      # "never": every Hyena block hands its operator a channel-last projection
 
